@@ -16,7 +16,9 @@
  * Element types (`dtype`): L2K_F32, L2K_F16, L2K_BF16. Arithmetic is fp32 in
  * every kernel; 16-bit types are rounded to nearest-even on store. The fp8
  * K/V cache entries (l2k_*_fp8_*) store cache elements as e4m3 bytes with a
- * per-cache fp32 scale (value = scale * e4m3) next to 16-bit activations.
+ * per-cache fp32 scale (value = scale * e4m3) next to 16-bit activations. The
+ * int8 entries (l2k_*_int8) hold rows of signed bytes with an fp32 scale per
+ * row (value = scale * byte) next to activations of any of the three types.
  */
 #ifndef LLAMA2_B200_H
 #define LLAMA2_B200_H
@@ -604,8 +606,52 @@ int l2k_decode_step_attention_paged(const l2k_decode_step_args *args, const uint
 int l2k_decode_step_no_alloc(const l2k_decode_step_args *args, l2k_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * 8-bit weights and activations (W8A8). No counterpart in the reference,
+ * whose kernels have no INT8 instantiation (its DataType names one,
+ * include/common/types.h:60-71); each replaces the operator named beside it.
+ * An int8 row holds signed bytes q in [-127, 127] and one fp32 scale:
+ *   a = max |y_j|,  scale = a / 127,  q_j = the integer nearest 127 y_j / a
+ * (ties to even; q does not depend on the order of any sum). A row of zeros,
+ * or without elements, has q = 0 and scale 0; a row that holds a NaN or an
+ * infinity has q = 0 and scale NaN, so every product of it is NaN. All tensors
+ * are row-major and contiguous except the operands of l2k_linear_int8, which
+ * have row strides. 16-byte aligned tensors with rows of a multiple of 8
+ * elements (16 bytes for l2k_linear_int8's operands) run fastest; any other
+ * alignment and length works.
+ *
+ * l2k_quantize_rows_int8: y = x, x (num_rows, dim), q (num_rows, dim),
+ *   scales (num_rows). For the attention output before the O projection, and
+ *   for weights: rows [out, in] give one scale per output channel.
+ * l2k_fused_add_residual_rmsnorm_int8: l2k_fused_add_residual_rmsnorm with
+ *   the normed row as int8: if add_residual, x = x + residual (written back
+ *   to x, rounded to dtype); y = x * weights / sqrt(mean(x^2) + 1e-5), not
+ *   rounded to dtype. residual is read only (may be NULL without
+ *   add_residual). As in that operator the squares are summed in fp32: a row
+ *   whose sum leaves its range has 1/rms 0, here scale 0.
+ * l2k_swiglu_int8: l2k_swiglu with the output row as int8, y in fp32 not
+ *   rounded to dtype.
+ * l2k_linear_int8: l2k_linear with trans_b on int8 operands:
+ *   c[i, j] = (sum_k a[i, k] b[j, k]) * (a_scales[i] * b_scales[j]),
+ *   a (m, k) with row stride lda, b (n, k) with row stride ldb (a weight
+ *   [out, in]), c (m, n) of type dtype with row stride ldc. The integer sum is
+ *   exact (k <= 131071, else L2K_ERR_UNSUPPORTED_SHAPE; bytes may be any value
+ *   from -128 to 127). tcgen05 tensor cores when a and b and their row strides
+ *   are multiples of 16 bytes, the CUDA cores otherwise; same results.
+ * ------------------------------------------------------------------------ */
+int l2k_quantize_rows_int8(const void *x, int8_t *q, float *scales, int64_t num_rows, int64_t dim, int dtype,
+                           l2k_stream_t stream);
+int l2k_fused_add_residual_rmsnorm_int8(const void *weights, void *x, const void *residual, int8_t *q, float *scales,
+                                        int64_t num_tokens, int64_t embed_dim, int add_residual, int dtype,
+                                        l2k_stream_t stream);
+int l2k_swiglu_int8(const void *input, int8_t *q, float *scales, int64_t num_tokens, int64_t intermediate_size,
+                    int dtype, l2k_stream_t stream);
+int l2k_linear_int8(int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t lda, const float *a_scales,
+                    const int8_t *b, int64_t ldb, const float *b_scales, void *c, int64_t ldc, int dtype,
+                    l2k_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Device-side error code recorded by kernels that wait on mbarriers (the
- * tcgen05 prefill scores, the streaming score rows, the fused decode step):
+ * tcgen05 prefill scores and GEMMs, the streaming score rows, the fused decode step):
  * 0 = none. Every such wait is bounded; a wait that
  * expires records its code here and the kernel exits instead of hanging.
  * Synchronizes with the device. clear != 0 resets the code. Returns -1 if

@@ -94,6 +94,10 @@ SIGNATURES = {
     "l2k_decode_step_attention_paged": [ctypes.POINTER(DecodeStepArgs), vp, i64, i64, vp, vp, vp],
     "l2k_decode_step_attention_no_alloc": [ctypes.POINTER(DecodeStepArgs), vp, vp],
     "l2k_decode_step_no_alloc": [ctypes.POINTER(DecodeStepArgs), vp],
+    "l2k_quantize_rows_int8": [vp, vp, vp, i64, i64, cint, vp],
+    "l2k_fused_add_residual_rmsnorm_int8": [vp, vp, vp, vp, vp, i64, i64, cint, cint, vp],
+    "l2k_swiglu_int8": [vp, vp, vp, i64, i64, cint, vp],
+    "l2k_linear_int8": [i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, i64, cint, vp],
     "l2k_device_error": ([cint], cint),
 }
 

@@ -567,6 +567,80 @@ def prefill_attention_scores(q, k, q_lens, kv_lens, max_q_len, max_kv_len, qk):
 
 
 # --------------------------------------------------------------------------
+# 8-bit weights and activations (W8A8): int8 rows with one fp32 scale per row
+# --------------------------------------------------------------------------
+def _int8_rows(q, scales, n, dim, name):
+    """Checks an int8 row tensor (n, dim) and its scales (n)."""
+    _require(q.dtype == torch.int8, f"{name} must be an int8 tensor, got {q.dtype}")
+    _require(scales.dtype == torch.float32, f"the scales of {name} must be float32, got {scales.dtype}")
+    _require(tuple(q.shape) == (n, dim), f"Incorrect {name} size")
+    _require(tuple(scales.shape) == (n,), f"Incorrect size of the scales of {name}")
+
+
+def _one_device(*ts):
+    """The CUDA device that all the tensors are on, made current for the call."""
+    for t in ts[1:]:
+        if t.device != ts[0].device:
+            raise ValueError(f"tensors are on different devices: {ts[0].device} and {t.device}")
+    return torch.cuda.device(ts[0].device)
+
+
+def launch_quantize_rows_int8(x, q, scales):
+    """Rows to int8: q (N, D) int8 and scales (N,) float32 with
+    x[i, j] ~ scales[i] * q[i, j], scales[i] = max_j |x[i, j]| / 127."""
+    _dev(x, q, scales)
+    n, dim = x.shape
+    _int8_rows(q, scales, n, dim, "q")
+    with _one_device(x, q, scales):
+        capi.call("l2k_quantize_rows_int8", x.data_ptr(), q.data_ptr(), scales.data_ptr(), n, dim, _code(x), _stream())
+
+
+def launch_fused_add_residual_rmsnorm_int8(weights, x, residual, q, scales, add_residual: bool):
+    """launch_fused_add_residual_rmsnorm with the normed rows as int8 (q, scales):
+    x is updated in place with add_residual; residual is read only (None
+    without add_residual)."""
+    ts = (weights, x, q, scales) + ((residual,) if add_residual else ())
+    _dev(*ts)
+    _same(x, weights, "launch_fused_add_residual_rmsnorm_int8")
+    n, dim = x.shape
+    if add_residual:
+        _same(x, residual, "launch_fused_add_residual_rmsnorm_int8")
+        _require(tuple(residual.shape) == (n, dim), "Incorrect residual size")
+    _require(tuple(weights.shape) == (dim,), "Incorrect rmsnorm weight size")
+    _int8_rows(q, scales, n, dim, "q")
+    with _one_device(*ts):
+        capi.call("l2k_fused_add_residual_rmsnorm_int8", weights.data_ptr(), x.data_ptr(),
+                  residual.data_ptr() if add_residual else None, q.data_ptr(), scales.data_ptr(), n, dim,
+                  int(bool(add_residual)), _code(x), _stream())
+
+
+def launch_swiglu_int8(input, q, scales):
+    """launch_swiglu with the output rows as int8: input (N, 2F) -> q (N, F), scales (N,)."""
+    _dev(input, q, scales)
+    n, f = q.shape
+    _require(tuple(input.shape) == (n, 2 * f), "Incorrect input size")
+    _int8_rows(q, scales, n, f, "q")
+    with _one_device(input, q, scales):
+        capi.call("l2k_swiglu_int8", input.data_ptr(), q.data_ptr(), scales.data_ptr(), n, f, _code(input), _stream())
+
+
+def launch_linear_int8(A, a_scales, B, b_scales, C):
+    """C = (A B^T) * a_scales[:, None] * b_scales[None, :] for int8 rows: A (M, K)
+    with a scale per token, B (N, K) (a weight [out, in]) with a scale per output
+    channel, C (M, N) float32, float16 or bfloat16; exact integer sums."""
+    _dev(A, a_scales, B, b_scales, C)
+    _require(A.dim() == 2 and B.dim() == 2 and C.dim() == 2, "Matrix dim do not match")
+    m, k = A.shape
+    n = B.shape[0]
+    _int8_rows(A, a_scales, m, k, "A")
+    _int8_rows(B, b_scales, n, k, "B")
+    _require(tuple(C.shape) == (m, n), "Incorrect C size")
+    with _one_device(A, a_scales, B, b_scales, C):
+        capi.call("l2k_linear_int8", m, n, k, A.data_ptr(), k, a_scales.data_ptr(), B.data_ptr(), k,
+                  b_scales.data_ptr(), C.data_ptr(), n, _code(C), _stream())
+
+
+# --------------------------------------------------------------------------
 # Fused decode step (one launch for the whole decode chain)
 # --------------------------------------------------------------------------
 def decode_step_workspace(device) -> torch.Tensor:

@@ -56,13 +56,16 @@ struct Int8Args
     void *c;
     int64_t ldc;
     int64_t m, n, k;
-    int n_kb;   // k blocks
-    int n_nt;   // column tiles
-    int bn;     // tile kernel: columns per tile (a multiple of 32)
-    int split;  // tile kernel: CTAs per cluster sharing one C tile, each a K range
-    int stages; // tile kernel: ring depth
-    int a_rows; // tile kernel: rows of the A box (the tile's other rows are never stored)
-    int wide;   // C rows are 16-byte aligned: 16-byte stores
+    int n_kb; // k blocks
+    int n_nt; // pair kernel: column tiles
+    int wide; // C rows are 16-byte aligned: 16-byte stores
+    // tile kernel
+    int bn;                           // columns per tile (a multiple of 32)
+    int split;                        // CTAs per cluster sharing one C tile, each a K range
+    int kb_per, kb_more;              // k blocks per rank; ranks that take one more
+    int groups;                       // rings and accumulators per CTA
+    int stages;                       // stages of all rings
+    uint32_t stage_bytes, ring_bytes; // (TileShape)
 };
 
 // kind::i8: D s32 (2), A and B signed (1), both K-major.
@@ -94,15 +97,13 @@ __device__ __forceinline__ void cluster_barrier()
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr)
+// The same without ordering memory: only that every thread has got here.
+__device__ __forceinline__ void cluster_barrier_relaxed()
 {
-    int4 v;
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
+__device__ __forceinline__ int64_t ceil_div_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank)
 {
     uint32_t r;
@@ -110,74 +111,114 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank)
     return r;
 }
 
-// Columns [col, col + 32) of a row of C from their integer sums: two fp32
-// roundings (the sum beyond 2^24, the product with the scales, whose own
-// product is a third) and one to T.
-template <typename T>
-__device__ __forceinline__ void store_scaled(const Int8Args &a, const uint32_t (&r)[32], int64_t row, int64_t col,
-                                             float row_scale)
+// One thread of a converged warp, known to the compiler as one: the tensor-core
+// and TMA instructions behind it are issued once. Behind a comparison with a
+// thread index each took about 80 cycles to issue instead, which set the pace
+// of the k loop (900 cycles a block, whatever its size).
+__device__ __forceinline__ bool elect_one()
 {
-    constexpr int N = Vec16<T>::N;
-    T *out = static_cast<T *>(a.c) + row * a.ldc;
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// A whole warp's wait; the same answer in every lane. Bounded like mbar_wait,
+// whose clock and flag are read only when the phase is not complete yet.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const volatile int *abort_flag)
+{
+    bool ok = mbar_try(bar, parity);
+    if (!__all_sync(0xffffffffu, ok))
+        ok = __all_sync(0xffffffffu, ok || mbar_wait(bar, parity, abort_flag));
+    return ok;
+}
+
+// Columns [col, col + 8) of a row of C from their integer sums and b_scales: three
+// fp32 roundings (the sum beyond 2^24, the product of the scales, the product of
+// both) and one to T. `n`: columns of C from col on.
+template <typename T>
+__device__ __forceinline__ void store8(T *out, const uint32_t *r, float row_scale, const float *sb, int64_t n, bool wide)
+{
+    T o[8];
 #pragma unroll
-    for (int v = 0; v < 32 / N; ++v)
+    for (int e = 0; e < 8; ++e)
+        o[e] = from_f<T>(__fmul_rn((float)(int)r[e], __fmul_rn(row_scale, sb[e])));
+    if (wide && n >= 8)
     {
-        const int64_t cv = col + N * v;
-        if (cv >= a.n)
-            break;
-        if (a.wide && cv + N <= a.n)
-        {
-            Vec16<T> o;
+        uint4 w[sizeof(T) / 2];
+        __builtin_memcpy(w, o, sizeof(o));
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                o.v[e] = from_f<T>(__fmul_rn((float)(int)r[N * v + e], __fmul_rn(row_scale, __ldg(a.sb + cv + e))));
-            stg(out + cv, as_u4(o));
-        }
-        else
-        {
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+            stg(out + 16 / sizeof(T) * i, w[i]);
+    }
+    else
+    {
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (cv + e < a.n)
-                    out[cv + e] =
-                        from_f<T>(__fmul_rn((float)(int)r[N * v + e], __fmul_rn(row_scale, __ldg(a.sb + cv + e))));
-        }
+        for (int e = 0; e < 8; ++e)
+            if (e < n)
+                out[e] = o[e];
     }
 }
 
 // ---------------------------------------------------------------------------
-// One BM x bn tile per cluster. Thread 0 initialises the barriers and issues
-// the first stages' loads before tensor memory is allocated, so the first
-// tiles are in flight during the set-up. With split > 1 every rank writes its
-// integer partial tile to its own shared memory (the drained ring), and after
-// a cluster barrier each rank sums the 32-column chunks dealt to it over all
-// ranks' copies; a second barrier keeps every copy alive until its readers
-// are done. Integer sums do not depend on the split.
+// One BM x bn tile per cluster of `split` CTAs, each a K range. Within a CTA the
+// k blocks are dealt to `groups` (1, 2 or 4) of one producer and one MMA warp
+// each, with a ring and an accumulator of their own, because one warp needs
+// about 350 cycles for a block's wait, four MMAs and commit where the tensor
+// cores need 32 to 128 per MMA. A producer warp initialises its own barriers and
+// issues its first loads at once, before tensor memory is allocated. The
+// epilogue adds the accumulators; integer sums do not depend on the dealing.
+//
+// split > 1: every rank leaves its partial tile in its own shared memory (the
+// drained ring). After a cluster barrier each rank adds its rows [q rows_per,
+// (q + 1) rows_per) into rank q's copy with one bulk reduction, and rank q
+// scales and stores those rows once all have landed. A last barrier keeps every
+// copy alive until it has been read.
+//
+// The A box has a.a_rows rows (m rounded up to 8). The MMA reads BM: the rest is
+// whatever follows in shared memory (a stage lies BM rows from its end at the
+// latest) and only reaches accumulator rows that are never read.
 // ---------------------------------------------------------------------------
-constexpr int kTThreads = 256;
-constexpr int kTMaxStages = 16;
-constexpr int kTRing = 200 * 1024; // bytes of shared memory for the ring at most
-constexpr uint32_t kTTmemCols = 256;
+constexpr int kTThreads = 512;
+constexpr int kTMaxStages = 32;
+constexpr uint32_t kTRing = 208 * 1024; // bytes of shared memory for the ring at most
+constexpr int kTMaxSmem = 227 * 1024;
 
-template <int BM>
-struct TileCfg
+// Shared memory: the ring (or the staged partial tile), bn scales, the barriers,
+// the TMEM address and the abort flag.
+struct TileShape
 {
-    static constexpr uint32_t kATile = BM * 128;
-    static uint32_t stage_bytes(int bn) { return kATile + (uint32_t)bn * 128; }
-    static int stages(int bn) { return (int)std::min<uint32_t>(kTMaxStages, kTRing / stage_bytes(bn)); }
-    // the ring (or the staged partial tile), then the barriers
-    static uint32_t ring_bytes(int bn)
-    {
-        return std::max<uint32_t>(stages(bn) * stage_bytes(bn), (uint32_t)BM * (bn + 4) * 4 + 1008) & ~1023u;
-    }
-    static uint32_t smem_bytes(int bn) { return ring_bytes(bn) + 8 * (2 * kTMaxStages + 1) + 24; }
+    int bm, bn, split, groups, stages;
+    uint32_t stage_bytes, ring_bytes, smem_bytes;
+    int a_rows;
 };
+inline TileShape tile_shape(int64_t m, int bm, int bn, int split, int groups)
+{
+    TileShape t{bm, bn, split, groups, 0, 0, 0, 0, 0};
+    t.a_rows = (int)std::min<int64_t>(bm, ceil_div(m, 8) * 8);
+    t.stage_bytes = (uint32_t)(bn + t.a_rows) * 128;
+    const uint32_t slack = (uint32_t)(bm - t.a_rows) * 128; // what the last stage's MMAs read past its A rows
+    t.stages = (int)std::min<uint32_t>(kTMaxStages, (kTRing - slack) / t.stage_bytes) / groups * groups;
+    const uint32_t staged = split > 1 ? (uint32_t)bm * (bn + 4) * 4 : 0;
+    t.ring_bytes = (std::max(t.stages * t.stage_bytes + slack, staged) + 1023) & ~1023u;
+    t.smem_bytes = t.ring_bytes + 4 * (uint32_t)bn + 8 * (2 * kTMaxStages + 2) + 16;
+    return t;
+}
+
+// Adds `bytes` of this CTA's shared memory at `src` to another CTA's at `dst`
+// as 32-bit integers, signalling its mbarrier (both shared::cluster addresses).
+__device__ __forceinline__ void bulk_add_s32(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.reduce.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes.add.s32 [%0], [%1], %2, "
+                 "[%3];" ::"r"(dst),
+                 "r"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 
 template <typename T, int BM>
 __global__ void __launch_bounds__(kTThreads, 1)
     linear_int8_tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                            const __grid_constant__ Int8Args a, const uint32_t off_bar)
+                            const __grid_constant__ Int8Args a)
 {
-    constexpr uint32_t kATile = BM * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
     if (sbase & 1023u) // (the same in every CTA: the whole cluster leaves)
@@ -186,122 +227,194 @@ __global__ void __launch_bounds__(kTThreads, 1)
             atomicCAS(&g_int8_error, 0, ERR_INT8_SMEM_ALIGN);
         return;
     }
-    const int stages = a.stages, bn = a.bn, split = a.split;
-    const uint32_t stage_bytes = kATile + (uint32_t)bn * 128;
-    const uint32_t bar_full = sbase + off_bar;             // + 8 * stage: the stage's tiles landed
-    const uint32_t bar_freed = bar_full + 8 * kTMaxStages; // + 8 * stage: the MMAs reading it completed
-    const uint32_t bar_done = bar_freed + 8 * kTMaxStages; // every MMA completed
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + off_bar + 8 * (2 * kTMaxStages + 1));
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 2);
+    const int bn = a.bn, split = a.split, groups = a.groups;
+    const int depth = a.stages / groups; // stages of one group's ring
+    float *sb = reinterpret_cast<float *>(smem + a.ring_bytes);
+    const uint32_t bar_full = sbase + a.ring_bytes + 4 * bn; // + 8 * stage: the stage's tiles landed
+    const uint32_t bar_freed = bar_full + 8 * kTMaxStages;   // + 8 * stage: the MMAs reading it completed
+    const uint32_t bar_done = bar_freed + 8 * kTMaxStages;   // every group's MMAs completed
+    const uint32_t bar_red = bar_done + 8;                   // the other ranks' rows have been added
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + a.ring_bytes + 4 * bn + 8 * (2 * kTMaxStages + 2));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = (int)(blockIdx.x % split);
-    const int tile = (int)(blockIdx.x / split);
-    const int64_t row0 = (int64_t)(tile / a.n_nt) * BM;
-    const int64_t col0 = (int64_t)(tile % a.n_nt) * bn;
-    const int kb0 = (int)((int64_t)rank * a.n_kb / split);
-    const int n_kb = (int)((int64_t)(rank + 1) * a.n_kb / split) - kb0; // at least 1 (split <= n_kb)
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0); // (uniform, known as such)
+    const int rank = (int)blockIdx.x;
+    const int64_t row0 = (int64_t)blockIdx.z * BM, col0 = (int64_t)blockIdx.y * bn;
+    const int kb0 = rank * a.kb_per + min(rank, a.kb_more); // the first a.kb_more ranks take one k block more
+    const int n_kb = a.kb_per + (rank < a.kb_more ? 1 : 0); // at least `groups`
 
-    auto issue = [&](int kb) {
-        const int st = kb % stages;
-        const uint32_t dst = sbase + st * stage_bytes;
+    // warps 0 .. groups - 1: producers; warps 4 .. 3 + groups: MMA issuers
+    const int group = warp & 3;
+    const int count = group < groups ? (n_kb - group + groups - 1) / groups : 0; // the group's k blocks
+    auto issue = [&](int i, int slot) { // the group's i-th k block into its ring's slot
+        const int st = slot * groups + group;
+        const uint32_t dst = sbase + st * a.stage_bytes;
         const uint32_t bar = bar_full + 8 * st;
-        mbar_expect_tx(bar, (uint32_t)(a.a_rows + bn) * 128);
-        tma_load_3d(dst + kATile, &tm_b, (kb0 + kb) * kBK, (int)col0, 0, bar);
-        tma_load_3d(dst, &tm_a, (kb0 + kb) * kBK, (int)row0, 0, bar);
+        const int kx = (kb0 + i * groups + group) * kBK;
+        mbar_expect_tx(bar, a.stage_bytes);
+        tma_load_3d(dst, &tm_b, kx, (int)col0, 0, bar);
+        tma_load_3d(dst + (uint32_t)bn * 128, &tm_a, kx, (int)row0, 0, bar);
     };
-
-    int issued = 0; // thread 0: k blocks whose loads were issued
-    if (tid == 0)
+    int issued = 0; // producers: the group's k blocks whose loads were issued
+    constexpr int kAtOnce = 2;
+    if (warp < groups)
     {
-        for (int i = 0; i < stages; ++i)
+        if (lane < depth)
         {
-            mbar_init(bar_full + 8 * i, 1);
-            mbar_init(bar_freed + 8 * i, 1);
+            mbar_init(bar_full + 8 * (lane * groups + group), 1);
+            mbar_init(bar_freed + 8 * (lane * groups + group), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        mbar_init(bar_done, 1);
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (; issued < n_kb && issued < stages; ++issued)
-            issue(issued);
+        __syncwarp();
+        issued = min(min(count, depth), kAtOnce);
+        if (elect_one())
+            for (int i = 0; i < issued; ++i)
+                issue(i, i);
+        __syncwarp();
     }
-    if (warp == 1)
+    else if (warp == 8)
     {
+        if (elect_one())
+        {
+            mbar_init(bar_done, groups);
+            mbar_init(bar_red, 1);
+            *abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(kTTmemCols));
+                     "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    else if (warp > 8)
+        for (int i = tid - 9 * 32; i < bn; i += kTThreads - 9 * 32)
+            sb[i] = col0 + i < a.n ? __ldg(a.sb + col0 + i) : 0.f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (tid == 0)
+    if (warp < groups)
     {
-        // ---- producer: the rest of the ring ----
-        for (int kb = issued; kb < n_kb && !*abort_flag; ++kb)
+        // ---- producer: the rest of the group's k blocks ----
+        int slot = issued;
+        if (elect_one())
+            for (; slot < depth && slot < count; ++slot)
+                issue(slot, slot);
+        __syncwarp();
+        issued = min(count, depth);
+        uint32_t phase = 0;
+        slot = 0;
+        for (int i = issued; i < count; ++i)
         {
-            if (!mbar_wait(bar_freed + 8 * (kb % stages), ((kb / stages) - 1) & 1, abort_flag))
+            if (!warp_wait(bar_freed + 8 * (slot * groups + group), phase, abort_flag))
             {
                 int8_fail(ERR_INT8_WAIT_MMA, abort_flag);
                 break;
             }
-            issue(kb);
-            issued = kb + 1;
+            if (elect_one())
+                issue(i, slot);
+            __syncwarp();
+            issued = i + 1;
+            if (++slot == depth)
+            {
+                slot = 0;
+                phase ^= 1;
+            }
         }
     }
-    else if (tid == 32)
+    else if (warp >= 4 && warp < 4 + groups)
     {
         // ---- MMA issuer ----
         const uint32_t idesc = int8_instr_desc(BM, (uint32_t)bn);
-        for (int kb = 0; kb < n_kb && !*abort_flag; ++kb)
+        const uint32_t acc = tmem + (uint32_t)(group * bn);
+        int slot = 0, i = 0;
+        uint32_t phase = 0;
+        for (; i < count; ++i)
         {
-            const int st = kb % stages;
-            if (!mbar_wait(bar_full + 8 * st, (kb / stages) & 1, abort_flag))
+            const int st = slot * groups + group;
+            if (!warp_wait(bar_full + 8 * st, phase, abort_flag))
             {
                 int8_fail(ERR_INT8_WAIT_LOAD, abort_flag);
                 break;
             }
             tc_fence_after();
-            const uint32_t pa = sbase + st * stage_bytes, pb = pa + kATile;
+            if (elect_one())
+            {
+                const uint32_t pb = sbase + st * a.stage_bytes;
+                const uint64_t da = smem_desc(pb + (uint32_t)bn * 128), db = smem_desc(pb);
 #pragma unroll
-            for (int k = 0; k < kBK / 32; ++k)
-                mma_i8(tmem, smem_desc(pa + 32u * k), smem_desc(pb + 32u * k), idesc, (kb | k) ? 1u : 0u);
-            mma_commit(bar_freed + 8 * st);
+                for (int k = 0; k < kBK / 32; ++k) // 32 bytes on along the rows: 2 units of 16
+                    mma_i8(acc, da + 2u * k, db + 2u * k, idesc, (i | k) ? 1u : 0u);
+                mma_commit(bar_freed + 8 * st);
+                if (i + 1 == count)
+                    mma_commit(bar_done);
+            }
+            __syncwarp();
+            if (++slot == depth)
+            {
+                slot = 0;
+                phase ^= 1;
+            }
         }
-        mma_commit(bar_done);
+        if (i < count && elect_one())
+            mma_commit(bar_done); // after a failure: what was issued
+        __syncwarp();
     }
-    __syncwarp();
 
-    // warps w and w + 4 read TMEM lane quadrant w: row 32 w + lane of the tile,
-    // or (BM 64) row 16 w + lane in lanes 0-15; each takes every other chunk
-    const int quad = warp & 3, half = warp >> 2;
+    // warps of the same warp % 4 read TMEM lane quadrant warp % 4: row 32 quad + lane of the
+    // tile, or (BM 64) row 16 quad + lane in lanes 0-15; they share its chunks of 32 columns
+    const int quad = warp & 3, part = warp >> 2;
     const int lrow = BM == 64 ? 16 * quad + lane : 32 * quad + lane;
     const bool live = (BM == 128 || lane < 16) && row0 + lrow < a.m;
     const float row_scale = live ? __ldg(a.sa + row0 + lrow) : 0.f;
     if (!mbar_wait(bar_done, 0, abort_flag))
         int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
-    if (tid == 0 && *abort_flag)
+    if (*abort_flag && warp < groups && lane == 0)
     {
         // after a failure the copies and MMAs in flight land before the ring is reused
         const int quiet = 0;
-        for (int kb = std::max(0, issued - stages); kb < issued; ++kb)
-            mbar_wait(bar_full + 8 * (kb % stages), (kb / stages) & 1, &quiet);
+        for (int i = max(0, issued - depth); i < issued; ++i)
+            mbar_wait(bar_full + 8 * ((i % depth) * groups + group), (i / depth) & 1, &quiet);
         mbar_wait(bar_done, 0, &quiet);
     }
     __syncwarp();
     tc_fence_after();
-    const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16);
+    // the integer sums of accumulator columns [c0, c0 + 32) of this thread's row
+    auto load32 = [&](int c0, uint32_t(&r)[32]) {
+        const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)c0;
+        tmem_ld32_async(taddr, r);
+        if (groups == 1)
+        {
+            tmem_wait_ld();
+            return;
+        }
+#pragma unroll 1
+        for (int g = 1; g < groups; ++g)
+        {
+            uint32_t x[32];
+            tmem_ld32_async(taddr + (uint32_t)(g * bn), x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                r[e] += x[e];
+        }
+    };
     if (split == 1)
     {
+        T *out = static_cast<T *>(a.c) + (row0 + lrow) * a.ldc + col0;
 #pragma unroll 1
-        for (int c0 = 32 * half; c0 < bn; c0 += 64)
+        for (int c0 = 32 * part; c0 < bn; c0 += 128)
         {
             uint32_t r[32];
-            tmem_ld32_async(taddr + (uint32_t)c0, r);
-            tmem_wait_ld();
+            load32(c0, r);
             if (live && !*abort_flag)
-                store_scaled<T>(a, r, row0 + lrow, col0 + c0, row_scale);
+            {
+#pragma unroll
+                for (int v = 0; v < 32; v += 8)
+                    store8<T>(out + c0 + v, r + v, row_scale, sb + c0 + v, a.n - col0 - c0 - v, a.wide);
+            }
             __syncwarp();
         }
     }
@@ -311,13 +424,16 @@ __global__ void __launch_bounds__(kTThreads, 1)
         __syncthreads(); // (after a failure: the ring is quiet)
         tc_fence_after();
         const int stride = bn + 4; // integers per staged row (16-byte shift per row: no bank conflicts)
+        const int m_tile = (int)std::min<int64_t>(BM, a.m - row0);
+        const int rows_per = (m_tile + split - 1) / split;
+        auto rows_of = [&](int q) { return max(0, min(m_tile, (q + 1) * rows_per) - q * rows_per); };
+        const int mine = rows_of(rank);
         int *stage = reinterpret_cast<int *>(smem);
 #pragma unroll 1
-        for (int c0 = 32 * half; c0 < bn; c0 += 64)
+        for (int c0 = 32 * part; c0 < bn; c0 += 128)
         {
             uint32_t r[32];
-            tmem_ld32_async(taddr + (uint32_t)c0, r);
-            tmem_wait_ld();
+            load32(c0, r);
             if (live)
             {
                 int4 *dst = reinterpret_cast<int4 *>(stage + lrow * stride + c0);
@@ -327,49 +443,298 @@ __global__ void __launch_bounds__(kTThreads, 1)
             }
             __syncwarp();
         }
+        fence_proxy_async(); // the staged rows, before the bulk reductions from and to them
+        if (tid == 0 && mine > 0)
+            mbar_expect_tx(bar_red, (uint32_t)((split - 1) * mine * stride * 4));
+        __syncwarp();
         cluster_barrier(); // every rank's partial is in its shared memory
-        // the tile's (row, 32-column chunk) items, dealt over the cluster's threads
-        // so that a warp's lanes hold consecutive rows of one chunk
-        const int m_tile = (int)std::min<int64_t>(BM, a.m - row0);
-        const int items = (bn / 32) * BM;
+        if (warp < split && warp != rank && rows_of(warp) > 0 && elect_one())
+        {
+            const uint32_t src = sbase + (uint32_t)(warp * rows_per * stride) * 4;
+            bulk_add_s32(cluster_addr(src, (uint32_t)warp), src, (uint32_t)(rows_of(warp) * stride * 4),
+                         cluster_addr(bar_red, (uint32_t)warp));
+        }
+        __syncwarp();
+        if (mine > 0 && !mbar_wait(bar_red, 0, abort_flag))
+            int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
+        // this rank's rows in runs of 8 columns; a warp's lanes take neighbouring runs
+        const int runs = bn / 8, items = runs * mine;
         if (!*abort_flag)
-            for (int i = rank * kTThreads + tid; i < items; i += split * kTThreads)
+            for (int i = tid; i < items; i += kTThreads)
             {
-                const int rr = i % BM, c0 = (i / BM) * 32;
-                if (rr >= m_tile || col0 + c0 >= a.n)
-                    continue;
-                uint32_t r[32] = {};
-                const uint32_t off = smem_u32(stage + rr * stride + c0);
-#pragma unroll 1
-                for (int q = 0; q < split; ++q)
-                {
-                    const uint32_t peer = cluster_addr(off, (uint32_t)q);
-                    int4 x[8];
-#pragma unroll
-                    for (int v = 0; v < 8; ++v)
-                        x[v] = ld_cluster_i4(peer + 16 * v);
-#pragma unroll
-                    for (int v = 0; v < 8; ++v)
-                    {
-                        r[4 * v] += (uint32_t)x[v].x;
-                        r[4 * v + 1] += (uint32_t)x[v].y;
-                        r[4 * v + 2] += (uint32_t)x[v].z;
-                        r[4 * v + 3] += (uint32_t)x[v].w;
-                    }
-                }
-                store_scaled<T>(a, r, row0 + rr, col0 + c0, __ldg(a.sa + row0 + rr));
+                const int rr = rank * rows_per + i / runs, c = (i % runs) * 8;
+                uint32_t r[8];
+                *reinterpret_cast<int4 *>(r) = *reinterpret_cast<const int4 *>(stage + rr * stride + c);
+                *reinterpret_cast<int4 *>(r + 4) = *reinterpret_cast<const int4 *>(stage + rr * stride + c + 4);
+                store8<T>(static_cast<T *>(a.c) + (row0 + rr) * a.ldc + col0 + c, r, __ldg(a.sa + row0 + rr), sb + c,
+                          a.n - col0 - c, a.wide);
             }
         __syncwarp();
-        cluster_barrier(); // no rank leaves while another may still read its partial
+        cluster_barrier_relaxed(); // no rank leaves while another may still read its partial
     }
 
     // -------- teardown --------
     tc_fence_before();
     __syncthreads();
+    if (warp == 8)
+    {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Two SMs per 256 x 256 tile (tcgen05.mma.cta_group::2, M = 256, N = 256):
+// CTA rank r of the pair holds rows [128 r, 128 r + 128) of the A tile and of
+// the B tile in its shared memory, at the same offsets, and receives rows
+// [128 r, 128 r + 128) of the accumulator in its tensor memory. Warp 0 of each
+// CTA streams its halves through the ring, the loads completing on rank 0's
+// "full" barrier; warp 1 of rank 0 issues the MMAs and commits to both CTAs'
+// "empty" and "accumulator full" barriers; warps 2-9 of each CTA scale and
+// store their 128 rows while the next tile's MMAs fill the other accumulator,
+// and release theirs on rank 0's "accumulator empty" barrier. The pairs walk
+// the tiles persistently.
+// ---------------------------------------------------------------------------
+constexpr int kPThreads = 64 + 256;                 // producer warp, MMA warp, epilogue warps
+constexpr int kPStages = 6;
+constexpr uint32_t kPHalf = 128 * 128;              // one CTA's half of an operand: 128 rows x 128 k
+constexpr uint32_t kPStageBytes = 2 * kPHalf;
+constexpr uint32_t kPOffScales = kPStages * kPStageBytes; // 128 b_scales per epilogue warp
+constexpr uint32_t kPOffBar = kPOffScales + 8 * 128 * 4;
+constexpr uint32_t kPOffMisc = kPOffBar + 8 * (2 * kPStages + 4);
+constexpr uint32_t kPSmemBytes = kPOffMisc + 16;
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar_cluster)
+{
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+                 "{%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar_cluster)
+                 : "memory");
+}
+// Arrives on the mbarrier at `bar` (same offset) in both CTAs of the pair once
+// the MMAs issued so far have completed.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
+                     "r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPThreads, 1)
+    linear_int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                            const __grid_constant__ Int8Args a)
+{
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sbase = smem_u32(smem);
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const bool leader = rank == 0;
+    const uint32_t bar_full = sbase + kPOffBar;             // + 8 * stage (rank 0's are the live ones)
+    const uint32_t bar_empty = bar_full + 8 * kPStages;     // + 8 * stage
+    const uint32_t bar_acc_full = bar_empty + 8 * kPStages; // + 8 * accumulator
+    const uint32_t bar_acc_empty = bar_acc_full + 16;       // + 8 * accumulator (rank 0's are the live ones)
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + kPOffMisc);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + kPOffMisc + 8);
+
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0); // (uniform, known as such)
+    const int64_t n_tiles = ceil_div_dev(a.m, 256) * a.n_nt;
+    const int64_t cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+    const int n_kb = a.n_kb;
+    const bool misaligned = (sbase & 1023u) != 0; // uniform over the cluster (same layout); acted on after the sync
+
+    if (tid == 0)
+    {
+        for (int i = 0; i < kPStages; ++i)
+        {
+            mbar_init(bar_full + 8 * i, 1);
+            mbar_init(bar_empty + 8 * i, 1);
+        }
+        for (int b = 0; b < 2; ++b)
+        {
+            mbar_init(bar_acc_full + 8 * b, 1);
+            mbar_init(bar_acc_empty + 8 * b, 2 * 8); // both CTAs' epilogue warps
+        }
+        *abort_flag = misaligned ? 1 : 0;
+        if (misaligned)
+            atomicCAS(&g_int8_error, 0, ERR_INT8_SMEM_ALIGN);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1)
+    {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier(); // both CTAs' barriers are initialized and the tensor memory allocated
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t full0 = cluster_addr(bar_full, 0);           // rank 0's full barriers
+    const uint32_t acc_empty0 = cluster_addr(bar_acc_empty, 0); // rank 0's accumulator-empty barriers
+
+    int64_t issued = 0;    // producer: k blocks whose loads were issued
+    int64_t mma_done = -1; // rank 0's MMA warp: the last k block whose MMAs were committed
+    if (warp == 0)
+    {
+        int st = 0;
+        uint32_t phase = 1; // (a fresh barrier's previous phase counts as complete)
+        for (int64_t tile = cluster_id; tile < n_tiles && !misaligned; tile += n_clusters)
+        {
+            const int row0 = (int)(tile / a.n_nt) * 256 + 128 * (int)rank;
+            const int col0 = (int)(tile % a.n_nt) * 256 + 128 * (int)rank;
+            int kb = 0;
+            for (; kb < n_kb; ++kb)
+            {
+                if (!warp_wait(bar_empty + 8 * st, phase, abort_flag))
+                {
+                    int8_fail(ERR_INT8_WAIT_MMA, abort_flag);
+                    break;
+                }
+                if (elect_one())
+                {
+                    const uint32_t dst = sbase + st * kPStageBytes;
+                    if (leader)
+                        mbar_expect_tx(bar_full + 8 * st, 2 * kPStageBytes); // both CTAs' halves
+                    tma_load_pair(dst, &tm_a, kb * kBK, row0, full0 + 8 * st);
+                    tma_load_pair(dst + kPHalf, &tm_b, kb * kBK, col0, full0 + 8 * st);
+                }
+                __syncwarp();
+                ++issued;
+                if (++st == kPStages)
+                {
+                    st = 0;
+                    phase ^= 1;
+                }
+            }
+            if (kb < n_kb)
+                break;
+        }
+    }
+    else if (warp == 1)
+    {
+        if (leader)
+        {
+            const uint32_t idesc = int8_instr_desc(256, 256);
+            int st = 0;
+            uint32_t phase = 0;
+            int64_t lt = 0;
+            for (int64_t tile = cluster_id; tile < n_tiles && !misaligned; tile += n_clusters, ++lt)
+            {
+                const int buf = (int)(lt & 1);
+                if (!warp_wait(bar_acc_empty + 8 * buf, (uint32_t)((lt >> 1) & 1) ^ 1u, abort_flag))
+                {
+                    int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem + (uint32_t)(buf * 256);
+                int kb = 0;
+                for (; kb < n_kb; ++kb)
+                {
+                    if (!warp_wait(bar_full + 8 * st, phase, abort_flag))
+                    {
+                        int8_fail(ERR_INT8_WAIT_LOAD, abort_flag);
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one())
+                    {
+                        const uint32_t pa = sbase + st * kPStageBytes;
+                        const uint64_t da = smem_desc(pa), db = smem_desc(pa + kPHalf);
+#pragma unroll
+                        for (int k = 0; k < kBK / 32; ++k) // 32 bytes on along the rows: 2 units of 16
+                            mma_i8_pair(acc, da + 2u * k, db + 2u * k, idesc, (kb | k) ? 1u : 0u);
+                        mma_commit_pair(bar_empty + 8 * st); // both CTAs may refill the stage
+                        if (kb + 1 == n_kb)
+                            mma_commit_pair(bar_acc_full + 8 * buf);
+                    }
+                    __syncwarp();
+                    ++mma_done;
+                    if (++st == kPStages)
+                    {
+                        st = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (kb < n_kb)
+                    break;
+            }
+        }
+    }
+    else
+    {
+        // epilogue warps 2..: TMEM lane quadrant warp % 4 holds rows 32 (warp % 4) + lane of this CTA's half;
+        // the two warps of a quadrant share its columns
+        const int quad = warp & 3, part = (warp - 2) >> 2;
+        float *sb = reinterpret_cast<float *>(smem + kPOffScales) + 128 * (warp - 2); // this warp's 128 columns
+        int64_t lt = 0;
+        for (int64_t tile = cluster_id; tile < n_tiles && !*abort_flag; tile += n_clusters, ++lt)
+        {
+            const int buf = (int)(lt & 1);
+            const int64_t row = (tile / a.n_nt) * 256 + 128 * (int64_t)rank + 32 * quad + lane;
+            const int64_t col0 = (tile % a.n_nt) * 256 + 128 * part;
+            const bool store = row < a.m;
+            const float row_scale = store ? __ldg(a.sa + row) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sb[32 * i + lane] = col0 + 32 * i + lane < a.n ? __ldg(a.sb + col0 + 32 * i + lane) : 0.f;
+            __syncwarp();
+            if (!mbar_wait(bar_acc_full + 8 * buf, (uint32_t)(lt >> 1) & 1u, abort_flag))
+            {
+                int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
+                break;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t taddr = tmem + (uint32_t)(buf * 256 + 128 * part) + ((uint32_t)(32 * quad) << 16);
+            T *out = static_cast<T *>(a.c) + row * a.ldc + col0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < 128; c0 += 32)
+            {
+                uint32_t r[32];
+                tmem_ld32_async(taddr + (uint32_t)c0, r);
+                tmem_wait_ld();
+                if (store)
+                {
+#pragma unroll
+                    for (int v = 0; v < 32; v += 8)
+                        store8<T>(out + c0 + v, r + v, row_scale, sb + c0 + v, a.n - col0 - c0 - v, a.wide);
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive_cluster(acc_empty0 + 8 * buf);
+        }
+    }
+
+    // -------- teardown: after a failure, copies and MMAs in flight land first --------
+    if (*abort_flag)
+    {
+        const int quiet = 0;
+        if (tid == 32 && leader && mma_done >= 0)
+            mbar_wait(bar_empty + 8 * (int)(mma_done % kPStages), (uint32_t)(mma_done / kPStages) & 1u, &quiet);
+        if (tid == 0 && leader)
+            for (int64_t it = issued > kPStages ? issued - kPStages : 0; it < issued; ++it)
+                mbar_wait(bar_full + 8 * (int)(it % kPStages), (uint32_t)(it / kPStages) & 1u, &quiet);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier(); // no CTA leaves while its peer may still signal its barriers or read its tensor memory
     if (warp == 1)
     {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
@@ -454,29 +819,33 @@ int launch_any(const Int8Args &a, cudaStream_t stream)
 }
 
 template <typename T, int BM>
-int launch_tile(Int8Args a, int bn, int split, cudaStream_t stream)
+int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
 {
-    using C = TileCfg<BM>;
+    while (groups > 1 && (groups * bn > 512 || groups > a.n_kb / split)) // 512 TMEM columns, a k block for each
+        groups /= 2;
+    const TileShape t = tile_shape(a.m, BM, bn, split, groups);
     a.bn = bn;
     a.split = split;
-    a.stages = C::stages(bn);
-    a.a_rows = (int)std::min<int64_t>(BM, ceil_div(a.m, 8) * 8);
-    a.n_nt = (int)ceil_div(a.n, bn);
+    a.kb_per = a.n_kb / split;
+    a.kb_more = a.n_kb % split;
+    a.groups = groups;
+    a.stages = t.stages;
+    a.stage_bytes = t.stage_bytes;
+    a.ring_bytes = t.ring_bytes;
     CUtensorMap ma, mb;
     const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const uint64_t m = (uint64_t)a.m, n = (uint64_t)a.n, k = (uint64_t)a.k, lda = (uint64_t)a.lda, ldb = (uint64_t)a.ldb;
-    if (!make_map(&ma, dt, a.a, k, m, 1, lda, lda * m, (uint32_t)a.a_rows, kBK) ||
+    if (!make_map(&ma, dt, a.a, k, m, 1, lda, lda * m, (uint32_t)t.a_rows, kBK) ||
         !make_map(&mb, dt, a.b, k, n, 1, ldb, ldb * n, (uint32_t)bn, kBK))
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
     auto kernel = linear_int8_tile_kernel<T, BM>;
-    const uint32_t smem = C::smem_bytes(bn);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTMaxSmem);
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ceil_div(a.m, BM) * a.n_nt * split));
+    cfg.gridDim = dim3((unsigned)split, (unsigned)ceil_div(a.n, bn), (unsigned)ceil_div(a.m, BM));
     cfg.blockDim = dim3(kTThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = t.smem_bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -485,10 +854,88 @@ int launch_tile(Int8Args a, int bn, int split, cudaStream_t stream)
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a, C::ring_bytes(bn));
+    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
     return check_launch("l2k_linear_int8");
+}
+
+// The two-SM kernel: 256 x 256 tiles over clusters of two CTAs.
+template <typename T>
+int launch_pair(Int8Args a, cudaStream_t stream)
+{
+    a.n_nt = (int)ceil_div(a.n, 256);
+    CUtensorMap ma, mb;
+    const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const uint64_t m = (uint64_t)a.m, n = (uint64_t)a.n, k = (uint64_t)a.k, lda = (uint64_t)a.lda, ldb = (uint64_t)a.ldb;
+    if (!make_map(&ma, dt, a.a, k, m, 1, lda, lda * m, 128, kBK) ||
+        !make_map(&mb, dt, a.b, k, n, 1, ldb, ldb * n, 128, kBK))
+        return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
+    auto kernel = linear_int8_pair_kernel<T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmemBytes);
+    if (e != cudaSuccess)
+        return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
+    const int64_t tiles = ceil_div(a.m, 256) * a.n_nt;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, num_sms() / 2)));
+    cfg.blockDim = dim3(kPThreads);
+    cfg.dynamicSmemBytes = kPSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
+    if (e != cudaSuccess)
+        return set_error(L2K_ERR_CUDA, "l2k_linear_int8 (two-SM tiles): %s", cudaGetErrorString(e));
+    return check_launch("l2k_linear_int8 (two-SM tiles)");
+}
+
+// Which kernel, and its tiles: the least estimated time, in clocks of an SM at
+// 1.9 GHz, from rates measured with these kernels on B200. A k block of a tile
+// takes the longest of its MMAs (bn / 2 each, for 64 and for 128 rows), its
+// issue (380 per warp) and its bytes at 56 per clock from L2; the whole product
+// at least its bytes at 3400 per clock from HBM. On top of that: 5000 for launch,
+// first loads and last stores, 3000 more for a reduction over a cluster, 18000 in
+// place of both for the two-SM kernel (whose tiles cover 2 SMs and end with 128
+// columns per warp to store).
+struct Plan
+{
+    int bm, bn, split, groups; // bm 256: the two-SM kernel
+};
+Plan plan(int64_t m, int64_t n, int n_kb)
+{
+    const int64_t sms = num_sms();
+    const double dram = ((double)m + n) * n_kb * kBK / 3400.0 + 2.0 * m * n / 3400.0;
+    Plan best{256, 256, 1, 1};
+    double best_t = std::max(dram, (double)ceil_div(ceil_div(m, 256) * ceil_div(n, 256), sms / 2) * n_kb * 585.0) + 18000.0;
+    const int bm = m <= 64 ? 64 : 128;
+    const int64_t mt = ceil_div(m, bm), a_rows = std::min<int64_t>(bm, ceil_div(m, 8) * 8);
+    if (mt * ceil_div(n, 256) > 4 * sms || mt > 65535 || ceil_div(n, 32) > 65535)
+        return best;
+    for (int bn = 32; bn <= 256; bn += 32)
+        for (int split = 1; split <= 8 && split <= n_kb; ++split)
+        {
+            const int64_t ctas = mt * ceil_div(n, bn) * split;
+            if (split > 1 && ctas > sms)
+                break;
+            const int per = (int)ceil_div(n_kb, split);
+            int groups = bn <= 64 && bm == 64 ? 4 : 2;
+            while (groups > 1 && groups > n_kb / split)
+                groups /= 2;
+            const double kb = std::max({2.0 * bn, 380.0 / groups, (double)(bn + a_rows) * 128 / 56.0});
+            const double t = std::max(dram, (double)ceil_div(ctas, sms) * (per * kb + 10.0 * bn)) + 5000.0 +
+                             (split > 1 ? 3000.0 : 0.0);
+            if (t < best_t)
+            {
+                best_t = t;
+                best = Plan{bm, bn, split, groups};
+            }
+        }
+    return best;
 }
 
 template <typename T>
@@ -501,9 +948,12 @@ int launch_linear(const Int8Args &p, cudaStream_t stream)
                     encode_fn() != nullptr;
     if (!tc)
         return launch_any<T>(a, stream);
-    if (a.m <= 64)
-        return launch_tile<T, 64>(a, 64, 1, stream);
-    return launch_tile<T, 128>(a, 128, 1, stream);
+    const Plan t = plan(a.m, a.n, a.n_kb);
+    if (t.bm == 64)
+        return launch_tile<T, 64>(a, t.bn, t.split, t.groups, stream);
+    if (t.bm == 128)
+        return launch_tile<T, 128>(a, t.bn, t.split, t.groups, stream);
+    return launch_pair<T>(a, stream);
 }
 
 } // namespace

@@ -12,24 +12,39 @@
 // q_j = rne(127 x_j w_j / max |x w|) and is left to the scale. x_j w_j is
 // exact in fp32 for 16-bit data and in fp64 for fp32 data, so q does not
 // depend on the order in which the squares are summed. SwiGLU's y is the fp32
-// value of silu_mul, not rounded to T first (one rounding fewer than
+// value of silu * up, not rounded to T first (one rounding fewer than
 // l2k_swiglu followed by l2k_quantize_rows_int8). Sums and maxima are fp32 or
 // wider.
 //
 // 127 y / a is evaluated as fma(y, 127 / a, 1.5 * 2^23), whose low byte is the
-// rounded integer: its error is below 127 * 2^-24 = 2^-17 (the rounded
-// reciprocal), so only values within 2^-14 of a border between two integers
-// can land on the wrong side; those few are divided in fp64.
+// rounded integer: its error is at most 127 * 2^-23 (the rounded reciprocal, and
+// y of fp64 products), so only values within 2^-14 of a border between two
+// integers can land on the wrong side; those are compared with the border in fp64.
+// Values of 16 bits need no second look (kShort).
+//
+// Three kernels:
+//   * rows_int8_stream_kernel, for many rows: CTAs stay on their SM and walk the
+//     rows; one thread keeps a ring of rows in flight with bulk copies into
+//     shared memory, so loads go on while a row is reduced and written (with a
+//     row's loads issued by the threads that then wait for its reduction, DRAM
+//     idled between them: 16384 x 4096 bf16 rows ran at 2.8 TB/s);
+//   * rows_int8_kernel, for few rows: one row per CTA, straight into registers;
+//   * rows_int8_any_kernel: rows longer than the others hold.
 #include "common.cuh"
+#include "tcgen05.cuh" // mbarriers
 
 #include <algorithm>
 #include <type_traits>
 
 namespace l2k
 {
+
+__device__ int g_int8_rows_error = 0; // first error code recorded by a kernel of this file
+
 namespace
 {
 
+constexpr int ERR_INT8_ROWS_WAIT = 0x801;
 constexpr float kRmsEps = 1e-5f;
 constexpr int kMaxThreads = 1024;
 
@@ -61,58 +76,81 @@ struct RowValue
         std::conditional_t<std::is_same<T, float>::value && (SRC == SRC_NORM || SRC == SRC_NORM_ADD), double, float>;
 };
 
-// |y| as an unsigned integer of the same order; NaN above infinity above all
-// finite values.
-__device__ __forceinline__ uint32_t mag_bits(float y) { return __float_as_uint(y) & 0x7fffffffu; }
-__device__ __forceinline__ uint64_t mag_bits(double y)
+// The largest |y| so far: fp32 with NaN above everything, or the bits of an fp64
+// (whose order, for magnitudes, is theirs as integers, NaN above infinity).
+struct TopF
 {
-    return (uint64_t)__double_as_longlong(y) & 0x7fffffffffffffffull;
-}
+    using Bits = uint32_t;
+    float v = 0.f;
+    __device__ __forceinline__ void add(float a, float b)
+    {
+        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(v), "f"(a), "f"(b));
+    }
+    __device__ __forceinline__ Bits bits() const { return __float_as_uint(v) & 0x7fffffffu; }
+};
+struct TopD
+{
+    using Bits = unsigned long long;
+    Bits v = 0;
+    __device__ __forceinline__ static Bits mag(double y)
+    {
+        return (Bits)__double_as_longlong(y) & 0x7fffffffffffffffull;
+    }
+    __device__ __forceinline__ void add(double a, double b) { v = max(v, max(mag(a), mag(b))); }
+    __device__ __forceinline__ Bits bits() const { return v; }
+};
+template <typename V>
+using Top = std::conditional_t<sizeof(V) == 8, TopD, TopF>;
+
 __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b); }
-__device__ __forceinline__ double from_bits(uint64_t b) { return __longlong_as_double((long long)b); }
+__device__ __forceinline__ double from_bits(unsigned long long b) { return __longlong_as_double((long long)b); }
 __device__ __forceinline__ bool finite_bits(uint32_t b) { return b < 0x7f800000u; }
-__device__ __forceinline__ bool finite_bits(uint64_t b) { return b < 0x7ff0000000000000ull; }
+__device__ __forceinline__ bool finite_bits(unsigned long long b) { return b < 0x7ff0000000000000ull; }
 __device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ uint64_t warp_max_bits(uint64_t v)
+__device__ __forceinline__ unsigned long long warp_max_bits(unsigned long long v)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
-        v = max((unsigned long long)v, (unsigned long long)__shfl_xor_sync(0xffffffffu, (unsigned long long)v, o));
+        v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
 // The largest magnitude and (norms) the sum of squares over the block; one
-// barrier, every thread gets both.
+// barrier, every thread gets both. A caller's consecutive rows alternate `buf`,
+// so that a warp that is a row ahead does not overwrite what another still reads.
 template <typename Bits, bool SUM>
-__device__ __forceinline__ void block_reduce(Bits &top, float &sq)
+__device__ __forceinline__ void block_reduce(Bits &top, float &sq, int buf)
 {
-    __shared__ Bits s_top[kMaxThreads / 32];
-    __shared__ float s_sq[kMaxThreads / 32];
+    __shared__ Bits s_top[2][kMaxThreads / 32];
+    __shared__ float s_sq[2][kMaxThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
     top = warp_max_bits(top);
     if (SUM)
         sq = warp_sum(sq);
     if (n_warps == 1)
+    {
+        __syncwarp();
         return;
+    }
     if (lane == 0)
     {
-        s_top[warp] = top;
+        s_top[buf][warp] = top;
         if (SUM)
-            s_sq[warp] = sq;
+            s_sq[buf][warp] = sq;
     }
     __syncthreads();
-    top = warp_max_bits(lane < n_warps ? s_top[lane] : Bits(0));
+    top = warp_max_bits(lane < n_warps ? s_top[buf][lane] : Bits(0));
     if (SUM)
-        sq = warp_sum(lane < n_warps ? s_sq[lane] : 0.f);
+        sq = warp_sum(lane < n_warps ? s_sq[buf][lane] : 0.f);
 }
 
 // What a row's values are divided by, and its scale.
 template <typename V>
 struct Quantizer
 {
-    V a;          // max |y| of the finite row, before 1 / rms
-    float r;      // 127 / a, or 0 where only the fp64 division is used
-    bool dead;    // every q of the row is 0
+    V a;           // max |y| of the row, before 1 / rms
+    float r, r_lo; // 127 / a to 48 bits; r = 0 where it or the values could leave the range of fp32
+    bool dead;     // every q of the row is 0
     float scale;
 };
 
@@ -122,57 +160,148 @@ __device__ __forceinline__ Quantizer<V> make_quantizer(Bits top, float inv_rms)
     Quantizer<V> z;
     z.a = from_bits(top);
     z.dead = !finite_bits(top) || top == 0;
-    // outside 2^-100 .. 2^100 the reciprocal or the values could leave the range of fp32
     z.r = !z.dead && z.a >= (V)0x1p-100 && z.a <= (V)0x1p100 ? (float)((V)127 / z.a) : 0.f;
+    z.r_lo = __fdividef(__fmaf_rn(-z.r, (float)z.a, 127.f), (float)z.a); // (of 16-bit a: an exact remainder)
     z.scale = finite_bits(top) ? (float)(z.a * (V)inv_rms / (V)127) : __uint_as_float(0x7fc00000u);
     return z;
 }
 
-// Correctly rounded 127 y / a: 127 y is exact in fp64 for fp32 y, and a
-// quotient of 24- and 32-bit integers that is no border between two integers
+// 127 y / a, correctly rounded: fp32 y have an exact product 127 y in fp64, and a
+// quotient of a 32- and a 24-bit integer that is no border between two integers
 // is further from one than fp64 rounds.
 template <typename V>
-__device__ __noinline__ int quantize_exact(V y, V a)
+__device__ __noinline__ uint32_t quantize_divided(V y, V a, bool dead)
 {
-    return __double2int_rn(__ddiv_rn(__dmul_rn((double)y, 127.0), (double)a));
+    return dead ? 0u : (uint32_t)__double2int_rn(__ddiv_rn(__dmul_rn((double)y, 127.0), (double)a));
 }
 
-// The 8-bit values of N consecutive y, packed low byte first.
-template <typename V, int N>
-__device__ __forceinline__ void quantize(const V (&y)[N], const Quantizer<V> &z, uint32_t (&bytes)[(N + 3) / 4])
+// The same for a value that lies next to the border k + 1/2, k >= 0: which side.
+__device__ __noinline__ uint32_t quantize_at_border(float y, float a, float r)
 {
-    constexpr float kMagic = 12582912.f; // 1.5 * 2^23: adding it rounds to an integer held in the low bits
-    uint32_t b[N];
-    float worst = 0.f;
-#pragma unroll
-    for (int e = 0; e < N; ++e)
+    const float k = floorf(fabsf(__fmul_rn(y, r)));
+    const double v = 127.0 * (double)fabsf(y), border = ((double)k + 0.5) * (double)a; // (31 and 32 bits: exact)
+    const int q = (int)k + (v > border || (v == border && ((int)k & 1)) ? 1 : 0);
+    return (uint32_t)(y < 0.f ? -q : q);
+}
+__device__ __forceinline__ uint32_t quantize_at_border(double y, double a, float)
+{
+    return quantize_divided(y, a, false);
+}
+
+// Two fp32 operations at once.
+__device__ __forceinline__ unsigned long long bits2(const float2 &v)
+{
+    unsigned long long u;
+    __builtin_memcpy(&u, &v, 8);
+    return u;
+}
+__device__ __forceinline__ float2 floats2(unsigned long long u)
+{
+    float2 v;
+    __builtin_memcpy(&v, &u, 8);
+    return v;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return floats2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return floats2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return floats2(d);
+}
+
+constexpr float kMagic = 12582912.f; // 1.5 * 2^23: adding it rounds to an integer held in the low bits
+constexpr float kBorder = 0.5f - 0x1p-14f;
+
+// Values of at most 16 bits (bf16 values and their products, f16 values) whose
+// row's largest has no more: 254 y and the odd multiples of a differ by more than
+// half a step of fp32 unless they are equal, so the fp32 nearest to 127 y / a is a
+// border k + 1/2 only where the quotient is, and adding kMagic then rounds ties to
+// even. 0.5 % of a bf16 row's values are ties: looking at each of them again cost
+// more than the whole fast path.
+template <typename T, int SRC>
+constexpr bool kShort = SRC != SRC_SWIGLU &&
+                        (std::is_same<T, __nv_bfloat16>::value || (std::is_same<T, __half>::value && SRC == SRC_ROWS));
+
+// The low byte of the result holds the 8-bit value of y.
+template <bool SHORT, typename V>
+__device__ __forceinline__ uint32_t quantize1(V y, const Quantizer<V> &z)
+{
+    if (z.r == 0.f)
+        return quantize_divided(y, z.a, z.dead);
+    if constexpr (SHORT)
+        return __float_as_uint(__fadd_rn(__fmaf_rn(y, z.r, __fmul_rn(y, z.r_lo)), kMagic));
+    else
     {
-        const float f = (float)y[e];
-        const float t = __fmaf_rn(f, z.r, kMagic);
-        worst = fmaxf(worst, fabsf(__fmaf_rn(f, z.r, -__fsub_rn(t, kMagic))));
-        b[e] = __float_as_uint(t);
+        const float t = __fmaf_rn((float)y, z.r, kMagic);
+        if (fabsf(__fmaf_rn((float)y, z.r, -__fsub_rn(t, kMagic))) > kBorder)
+            return quantize_at_border(y, z.a, z.r);
+        return __float_as_uint(t);
     }
-    if (z.dead)
+}
+
+// The 8-bit values of 8 consecutive y, packed low byte first.
+template <bool SHORT, typename V>
+__device__ __forceinline__ uint2 quantize8(const V (&y)[8], const Quantizer<V> &z)
+{
+    uint32_t b[8];
+    if (z.r == 0.f) // (the whole row)
     {
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            b[e] = 0;
+        for (int e = 0; e < 8; ++e)
+            b[e] = quantize_divided(y[e], z.a, z.dead);
     }
-    else if (worst > 0.5f - 0x1p-14f || z.r == 0.f)
+    else
     {
+        const float2 r2 = make_float2(z.r, z.r), magic2 = make_float2(kMagic, kMagic);
+        if constexpr (SHORT)
+        {
+            const float2 lo2 = make_float2(z.r_lo, z.r_lo);
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            b[e] = (uint32_t)quantize_exact(y[e], z.a);
-    }
+            for (int e = 0; e < 8; e += 2)
+            {
+                const float2 f = make_float2(y[e], y[e + 1]);
+                const float2 t = add2(fma2(f, r2, mul2(f, lo2)), magic2);
+                b[e] = __float_as_uint(t.x);
+                b[e + 1] = __float_as_uint(t.y);
+            }
+        }
+        else
+        {
+            const float2 minus2 = make_float2(-1.f, -1.f);
+            float off = 0.f; // the largest distance from the integer rounded to
 #pragma unroll
-    for (int i = 0; i < (N + 3) / 4; ++i)
-    {
-        uint32_t v = b[4 * i] & 0xffu;
-        if (4 * i + 3 < N)
-            v = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040),
-                            0x5410);
-        bytes[i] = v;
+            for (int e = 0; e < 8; e += 2)
+            {
+                const float2 f = make_float2((float)y[e], (float)y[e + 1]);
+                const float2 t = fma2(f, r2, magic2);
+                const float2 d = fma2(f, r2, fma2(t, minus2, magic2));
+                asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(off) : "f"(off), "f"(d.x), "f"(d.y));
+                b[e] = __float_as_uint(t.x);
+                b[e + 1] = __float_as_uint(t.y);
+            }
+            if (off > kBorder)
+            {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    b[e] = quantize1<false>(y[e], z);
+            }
+        }
     }
+    uint2 w;
+    w.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    w.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+    return w;
 }
 
 // 8 consecutive elements from a 16-byte aligned address.
@@ -191,29 +320,149 @@ __device__ __forceinline__ Raw8<T> load8(const T *p, bool keep)
     return r;
 }
 template <typename T>
+__device__ __forceinline__ Raw8<T> load8_shared(const uint8_t *p)
+{
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+        r.v[i] = *reinterpret_cast<const uint4 *>(p + 16 * i);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const Raw8<T> &r)
+{
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+        stg(p + 16 / sizeof(T) * i, r.v[i]);
+}
+// The same values, unknown as such to the compiler.
+template <typename T>
+__device__ __forceinline__ void opaque(Raw8<T> &r)
+{
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+        asm("" : "+r"(r.v[i].x), "+r"(r.v[i].y), "+r"(r.v[i].z), "+r"(r.v[i].w));
+}
+template <typename T>
 __device__ __forceinline__ void unpack8(const Raw8<T> &r, T (&v)[8])
 {
     __builtin_memcpy(v, &r, sizeof(r));
 }
 
-// One row per CTA, held in registers: thread t takes the groups of 8 elements
-// t, t + blockDim.x, ... (NV of them at most).
+// silu(g) * u in fp32 by the fast exponential and reciprocal, for every type: their
+// errors (2 + 1.2 |g| steps of fp32 and 1) are 1e-6 of an 8-bit row's step. 0
+// where exp(-g) leaves the range of fp32 (g < -87), as in l2k_swiglu.
+__device__ __forceinline__ float silu_up(float g, float u)
+{
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(e, 1.0f)));
+    return __fmul_rn(__fmul_rn(g, r), u);
+}
+
+// y of 8 elements of a row (or with ADD of the sum to write back) and the norm's weights.
+template <typename T, int SRC, typename V>
+__device__ __forceinline__ void values8(const Raw8<T> &in, const Raw8<T> &w, V (&y)[8])
+{
+    T v[8], u[8];
+    unpack8(in, v);
+    unpack8(w, u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        y[e] = SRC == SRC_ROWS ? (V)to_f(v[e]) : (V)to_f(v[e]) * (V)to_f(u[e]);
+}
+
+// What a thread holds of 8 elements from the first look at them to the second:
+// SwiGLU's y, and fp64 products where the registers allow (NV <= 2: 133 us for
+// 16384 x 4096 fp32 norms, 154 when they are computed twice); else the inputs, half
+// the registers or less, from which y is computed again.
+template <typename T, int SRC, int NV>
+struct Held
+{
+    using V = typename RowValue<T, SRC>::type;
+    static constexpr bool kNorm = SRC == SRC_NORM || SRC == SRC_NORM_ADD;
+    static constexpr bool kKeep = SRC == SRC_SWIGLU || (sizeof(V) == 8 && NV <= 2);
+    Raw8<T> in;
+    V y[8];
+
+    // The first look: in2 is the residual, or SwiGLU's up half; with ADD `in`
+    // becomes the sum to write back.
+    __device__ __forceinline__ void look(const Raw8<T> &first, const Raw8<T> &in2, const Raw8<T> &w, Top<V> &top, float &sq)
+    {
+        T v[8], u[8];
+        unpack8(first, v);
+        if constexpr (SRC == SRC_SWIGLU)
+        {
+            unpack8(in2, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[e] = silu_up(to_f(v[e]), to_f(u[e]));
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                top.add(y[e], y[e + 1]);
+        }
+        else
+        {
+            if constexpr (SRC == SRC_NORM_ADD)
+            {
+                unpack8(in2, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = from_f<T>(__fadd_rn(to_f(v[e]), to_f(u[e])));
+            }
+            __builtin_memcpy(&in, v, sizeof(in));
+            if constexpr (kNorm)
+            {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sq = fmaf(to_f(v[e]), to_f(v[e]), sq);
+            }
+            V t[8];
+            values8<T, SRC>(in, w, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (kKeep)
+                    y[e] = t[e];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                top.add(t[e], t[e + 1]);
+        }
+    }
+    __device__ __forceinline__ uint2 quantized(const Raw8<T> &w, const Quantizer<V> &z) const
+    {
+        if constexpr (kKeep)
+            return quantize8<false>(y, z);
+        else
+        {
+            V t[8];
+            Raw8<T> again = in, w_again = w;
+            opaque(again); // (else the compiler keeps the first look's products instead)
+            opaque(w_again);
+            values8<T, SRC>(again, w_again, t);
+            return quantize8<kShort<T, SRC>>(t, z);
+        }
+    }
+};
+
+__device__ __forceinline__ float inv_rms_of(float sq, int64_t dim)
+{
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sq, (float)dim), kRmsEps)));
+}
+
+// One row per CTA: thread t takes the groups of 8 elements t, t + blockDim.x, ...
+// (NV of them at most).
 template <typename T, int SRC, int NV>
 __global__ void __launch_bounds__(kMaxThreads) rows_int8_kernel(const RowArgs a)
 {
     using V = typename RowValue<T, SRC>::type;
-    using Bits = std::conditional_t<sizeof(V) == 8, uint64_t, uint32_t>;
     constexpr bool kNorm = SRC == SRC_NORM || SRC == SRC_NORM_ADD;
     const int64_t row = blockIdx.x;
     const int n_groups = (int)(a.dim / 8);
     const T *src = static_cast<const T *>(kNorm ? a.xio : a.x) + row * a.dim * (SRC == SRC_SWIGLU ? 2 : 1);
     const T *add = SRC == SRC_NORM_ADD ? static_cast<const T *>(a.residual) + row * a.dim : nullptr;
-    const T *w = static_cast<const T *>(a.w);
+    T *xio = static_cast<T *>(a.xio) + row * a.dim;
 
-    V y[NV][8];
-    Bits top = 0;
-    float sq = 0.f;
-    Raw8<T> in[NV], in2[NV];
+    Raw8<T> in[NV], in2[NV], w[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
     {
@@ -225,88 +474,310 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_kernel(const RowArgs a)
                 in2[j] = load8(add + 8 * g, false);
             if (SRC == SRC_SWIGLU)
                 in2[j] = load8(src + a.dim + 8 * g, false);
+            if (kNorm)
+                w[j] = load8(static_cast<const T *>(a.w) + 8 * g, true);
         }
     }
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-    {
-        const int g = threadIdx.x + j * blockDim.x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            y[j][e] = (V)0;
-        if (g >= n_groups)
-            continue;
-        T v[8], u[8];
-        unpack8(in[j], v);
-        if constexpr (SRC == SRC_ROWS)
-        {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                y[j][e] = to_f(v[e]);
-        }
-        else if constexpr (SRC == SRC_SWIGLU)
-        {
-            unpack8(in2[j], u);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                y[j][e] = silu_mul<T>(to_f(v[e]), to_f(u[e]));
-        }
-        else
-        {
-            if constexpr (SRC == SRC_NORM_ADD)
-            {
-                unpack8(in2[j], u);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    v[e] = from_f<T>(__fadd_rn(to_f(v[e]), to_f(u[e])));
-                Raw8<T> o;
-                __builtin_memcpy(&o, v, sizeof(o));
-                T *dst = static_cast<T *>(a.xio) + row * a.dim + 8 * g;
-#pragma unroll
-                for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-                    stg(dst + 16 / sizeof(T) * i, o.v[i]);
-            }
-            unpack8(load8(w + 8 * g, true), u);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                const float f = to_f(v[e]);
-                sq = fmaf(f, f, sq);
-                y[j][e] = (V)f * (V)to_f(u[e]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            top = max(top, mag_bits(y[j][e]));
-    }
-    block_reduce<Bits, kNorm>(top, sq);
-    float inv_rms = 1.f;
-    if (kNorm)
-        inv_rms = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sq, (float)a.dim), kRmsEps)));
-    const Quantizer<V> z = make_quantizer<V>(top, inv_rms);
-    int8_t *q = a.q + row * a.dim;
+    Held<T, SRC, NV> held[NV];
+    Top<V> top;
+    float sq = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
     {
         const int g = threadIdx.x + j * blockDim.x;
         if (g < n_groups)
         {
-            uint32_t b[2];
-            quantize<V, 8>(y[j], z, b);
-            *reinterpret_cast<uint2 *>(q + 8 * g) = make_uint2(b[0], b[1]);
+            held[j].look(in[j], in2[j], w[j], top, sq);
+            if (SRC == SRC_NORM_ADD)
+                store8(xio + 8 * g, held[j].in);
         }
+    }
+    auto bits = top.bits();
+    block_reduce<decltype(bits), kNorm>(bits, sq, 0);
+    const Quantizer<V> z = make_quantizer<V>(bits, kNorm ? inv_rms_of(sq, a.dim) : 1.f);
+    int8_t *q = a.q + row * a.dim;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+    {
+        const int g = threadIdx.x + j * blockDim.x;
+        if (g < n_groups)
+            *reinterpret_cast<uint2 *>(q + 8 * g) = held[j].quantized(w[j], z);
     }
     if (threadIdx.x == 0)
         a.scales[row] = z.scale;
 }
 
-// Any length and alignment: two passes over the row, an element at a time
-// (the second re-reads it, normally from L1 or L2, and recomputes y).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// The rows blockIdx.x, blockIdx.x + gridDim.x, ... through a ring of `depth`
+// stages, each one row's inputs (x, then the residual; or SwiGLU's gate and up
+// halves). A stage is refilled once the row's reduction has shown that every
+// thread has read it. Each thread holds NV groups of 8 elements.
+//
+// Aligned rows (16-byte aligned, a multiple of 8 elements): groups of 8
+// neighbours, 16-byte accesses. RAGGED: rows of any length and alignment. The copy
+// takes the 16-byte units that the row touches (bytes of the rows next to it are
+// not used), except units that reach out of the tensor, whose elements are read
+// from global memory; element i of group j of thread t is (8 j + i) threads + t,
+// so that a warp's element accesses are to neighbours.
+constexpr int kMaxDepth = 8;
+constexpr int kStreamThreads = 512;
+constexpr int kTwoPerSM = 448; // threads of the instantiation held to 72 registers, so that an SM takes two CTAs
+
+__device__ __forceinline__ uintptr_t down16(uintptr_t p) { return p & ~(uintptr_t)15; }
+__device__ __forceinline__ uintptr_t up16(uintptr_t p) { return (p + 15) & ~(uintptr_t)15; }
+
+// One input of a ragged row: where its bytes are and which of them are copied.
+struct RaggedRow
+{
+    uintptr_t begin, lo, hi; // the row's first byte; the copied bytes [lo, hi)
+    bool clipped;            // some of its units reach out of the tensor
+    __device__ __forceinline__ RaggedRow(const void *base, int64_t row, int64_t row_bytes, int64_t n_rows)
+    {
+        const uintptr_t first = (uintptr_t)base, end = first + n_rows * row_bytes;
+        begin = first + row * row_bytes;
+        lo = down16(begin);
+        hi = up16(begin + row_bytes);
+        clipped = lo < first || hi > end;
+        if (clipped)
+        {
+            lo = lo < first ? up16(first) : lo;
+            hi = hi > end ? down16(end) : hi;
+            hi = hi > lo ? hi : lo;
+        }
+    }
+    // Elements `stride` apart from the e-th on, those below `end`; zeros for the rest.
+    template <typename T>
+    __device__ __forceinline__ Raw8<T> load(const uint8_t *stage, int e, int stride, int end) const
+    {
+        const T *p = reinterpret_cast<const T *>(stage + (begin & 15));
+        T v[8];
+        if (!clipped && e + 7 * stride < end)
+        {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = p[e + i * stride];
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                const int x = e + i * stride;
+                const uintptr_t g = begin + (int64_t)x * sizeof(T);
+                v[i] = x >= end ? from_f<T>(0.f) : g >= lo && g < hi ? p[x] : *reinterpret_cast<const T *>(g);
+            }
+        }
+        Raw8<T> r;
+        __builtin_memcpy(&r, v, sizeof(r));
+        return r;
+    }
+};
+
+// Values into elements `stride` apart from the e-th on, those below `end`.
+template <typename B>
+__device__ __forceinline__ void scatter8(B *p, const B (&v)[8], int e, int stride, int end)
+{
+    if (e + 7 * stride < end)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            p[e + i * stride] = v[i];
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (e + i * stride < end)
+                p[e + i * stride] = v[i];
+    }
+}
+
+template <typename T, int SRC, int NV, bool RAGGED, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == kTwoPerSM ? 2 : 1)
+    rows_int8_stream_kernel(const RowArgs a, const int depth, const uint32_t input_bytes)
+{
+    using V = typename RowValue<T, SRC>::type;
+    constexpr bool kNorm = SRC == SRC_NORM || SRC == SRC_NORM_ADD;
+    constexpr int kCopies = SRC == SRC_NORM_ADD ? 2 : 1;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ __align__(8) uint64_t s_full[kMaxDepth];
+    __shared__ int s_abort;
+    const int tid = threadIdx.x, n_threads = blockDim.x;
+    const int dim = (int)a.dim;
+    const int64_t row_bytes = a.dim * (int64_t)sizeof(T) * (SRC == SRC_SWIGLU ? 2 : 1);
+    const void *const base = kNorm ? a.xio : a.x;
+    const uint32_t stage_bytes = input_bytes * kCopies;
+    const int64_t n_mine = (a.n_rows - blockIdx.x + gridDim.x - 1) / gridDim.x; // (gridDim.x <= n_rows)
+    auto issue = [&](int64_t it, int slot) {
+        const int64_t row = blockIdx.x + it * gridDim.x;
+        const uint32_t dst = smem_u32(ring) + slot * stage_bytes, bar = smem_u32(&s_full[slot]);
+        if constexpr (RAGGED)
+        {
+            const RaggedRow x(base, row, row_bytes, a.n_rows);
+            const RaggedRow r(kCopies == 2 ? a.residual : base, row, row_bytes, a.n_rows);
+            const uint32_t nx = (uint32_t)(x.hi - x.lo), nr = kCopies == 2 ? (uint32_t)(r.hi - r.lo) : 0;
+            mbar_expect_tx(bar, nx + nr);
+            if (nx)
+                bulk_load(dst + (uint32_t)(x.lo - down16(x.begin)), (const void *)x.lo, nx, bar);
+            if (nr)
+                bulk_load(dst + input_bytes + (uint32_t)(r.lo - down16(r.begin)), (const void *)r.lo, nr, bar);
+        }
+        else
+        {
+            mbar_expect_tx(bar, stage_bytes);
+            bulk_load(dst, static_cast<const uint8_t *>(base) + row * row_bytes, input_bytes, bar);
+            if (kCopies == 2)
+                bulk_load(dst + input_bytes, static_cast<const uint8_t *>(a.residual) + row * row_bytes, input_bytes, bar);
+        }
+    };
+    int64_t issued = n_mine < depth ? n_mine : depth; // (thread 0's)
+    if (tid == 0)
+    {
+        for (int i = 0; i < depth; ++i)
+            mbar_init(smem_u32(&s_full[i]), 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < (int)issued; ++i)
+            issue(i, i);
+    }
+    // the first element of group j, whose elements are `stride` apart
+    const int stride = RAGGED ? n_threads : 1;
+    auto at = [&](int j) { return RAGGED ? 8 * j * n_threads + tid : 8 * (j * n_threads + tid); };
+    Raw8<T> w[NV];
+    if (kNorm)
+    {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+        {
+            if constexpr (RAGGED)
+            {
+                T v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = at(j) + i * stride < dim ? static_cast<const T *>(a.w)[at(j) + i * stride] : from_f<T>(0.f);
+                __builtin_memcpy(&w[j], v, sizeof(v));
+            }
+            else if (at(j) < dim)
+                w[j] = load8(static_cast<const T *>(a.w) + at(j), true);
+        }
+    }
+    __syncthreads();
+    const volatile int *abort_flag = &s_abort;
+
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int64_t it = 0; it < n_mine; ++it)
+    {
+        const int64_t row = blockIdx.x + it * gridDim.x;
+        const uint32_t bar = smem_u32(&s_full[slot]);
+        if (!mbar_try(bar, phase) && !mbar_wait(bar, phase, abort_flag))
+        {
+            atomicCAS(&g_int8_rows_error, 0, ERR_INT8_ROWS_WAIT);
+            s_abort = 1;
+        }
+        const bool arrived = !*abort_flag; // (a row that has not arrived is not written back)
+        const uint8_t *stage = ring + slot * stage_bytes;
+        Held<T, SRC, NV> held[NV];
+        Top<V> top;
+        float sq = 0.f;
+        if constexpr (RAGGED)
+        {
+            const RaggedRow x(base, row, row_bytes, a.n_rows);
+            const RaggedRow r(kCopies == 2 ? a.residual : base, row, row_bytes, a.n_rows);
+            T *out = static_cast<T *>(a.xio) + row * a.dim;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+            {
+                const int e = at(j);
+                if (e >= dim)
+                    continue;
+                Raw8<T> in = x.template load<T>(stage, e, stride, dim), in2;
+                if (SRC == SRC_NORM_ADD)
+                    in2 = r.template load<T>(stage + input_bytes, e, stride, dim);
+                if (SRC == SRC_SWIGLU)
+                    in2 = x.template load<T>(stage, e + dim, stride, 2 * dim);
+                held[j].look(in, in2, w[j], top, sq); // (the zeros past the row add nothing)
+                if (SRC == SRC_NORM_ADD && arrived)
+                {
+                    T v[8];
+                    unpack8(held[j].in, v);
+                    scatter8(out, v, e, stride, dim);
+                }
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+            {
+                const int e = at(j);
+                if (e >= dim)
+                    continue;
+                const uint8_t *p = stage + (uint32_t)e * sizeof(T);
+                Raw8<T> in = load8_shared<T>(p), in2;
+                if (SRC == SRC_NORM_ADD)
+                    in2 = load8_shared<T>(p + input_bytes);
+                if (SRC == SRC_SWIGLU)
+                    in2 = load8_shared<T>(p + (uint32_t)dim * sizeof(T));
+                held[j].look(in, in2, w[j], top, sq);
+                if (SRC == SRC_NORM_ADD && arrived)
+                    store8(static_cast<T *>(a.xio) + row * a.dim + e, held[j].in);
+            }
+        }
+        auto bits = top.bits();
+        block_reduce<decltype(bits), kNorm>(bits, sq, (int)(it & 1));
+        if (*abort_flag)
+            break; // (set before the barrier: the same answer in every thread)
+        if (tid == 0 && issued < n_mine)
+            issue(issued++, slot);
+        const Quantizer<V> z = make_quantizer<V>(bits, kNorm ? inv_rms_of(sq, a.dim) : 1.f);
+        int8_t *q = a.q + row * a.dim;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+        {
+            if (at(j) >= dim)
+                continue;
+            const uint2 b = held[j].quantized(w[j], z);
+            if constexpr (RAGGED)
+            {
+                int8_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = (int8_t)((i < 4 ? b.x : b.y) >> (8 * (i & 3)));
+                scatter8(q, v, at(j), stride, dim);
+            }
+            else
+                *reinterpret_cast<uint2 *>(q + at(j)) = b;
+        }
+        if (tid == 0)
+            a.scales[row] = z.scale;
+        if (++slot == depth)
+        {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+    if (*abort_flag && tid == 0)
+    {
+        // after a failure the copies in flight land before the CTA leaves
+        const int quiet = 0;
+        for (int64_t i = issued > depth ? issued - depth : 0; i < issued; ++i)
+            mbar_wait(smem_u32(&s_full[i % depth]), (uint32_t)(i / depth) & 1u, &quiet);
+    }
+}
+
+// Any length: two passes over the row, an element at a time (the second re-reads
+// it, normally from L1 or L2, and recomputes y).
 template <typename T, int SRC>
 __global__ void __launch_bounds__(kMaxThreads) rows_int8_any_kernel(const RowArgs a)
 {
     using V = typename RowValue<T, SRC>::type;
-    using Bits = std::conditional_t<sizeof(V) == 8, uint64_t, uint32_t>;
     constexpr bool kNorm = SRC == SRC_NORM || SRC == SRC_NORM_ADD;
     const int64_t row = blockIdx.x;
     const T *src = static_cast<const T *>(kNorm ? a.xio : a.x) + row * a.dim * (SRC == SRC_SWIGLU ? 2 : 1);
@@ -315,13 +786,13 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_any_kernel(const RowArg
     T *xio = static_cast<T *>(a.xio) + row * a.dim;
     auto value = [&](int64_t d, float f) -> V {
         if constexpr (SRC == SRC_SWIGLU)
-            return silu_mul<T>(f, to_f(src[a.dim + d]));
+            return silu_up(f, to_f(src[a.dim + d]));
         else if constexpr (kNorm)
             return (V)f * (V)to_f(w[d]);
         else
             return f;
     };
-    Bits top = 0;
+    Top<V> top;
     float sq = 0.f;
     for (int64_t d = threadIdx.x; d < a.dim; d += blockDim.x)
     {
@@ -335,32 +806,77 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_any_kernel(const RowArg
         else
             f = to_f(src[d]);
         sq = fmaf(f, f, sq);
-        top = max(top, mag_bits(value(d, f)));
+        top.add(value(d, f), (V)0);
     }
-    block_reduce<Bits, kNorm>(top, sq);
-    float inv_rms = 1.f;
-    if (kNorm)
-        inv_rms = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sq, (float)a.dim), kRmsEps)));
-    const Quantizer<V> z = make_quantizer<V>(top, inv_rms);
+    auto bits = top.bits();
+    block_reduce<decltype(bits), kNorm>(bits, sq, 0);
+    const Quantizer<V> z = make_quantizer<V>(bits, kNorm ? inv_rms_of(sq, a.dim) : 1.f);
     int8_t *q = a.q + row * a.dim;
-    for (int64_t d = threadIdx.x; d < a.dim; d += blockDim.x)
-    {
-        // (with ADD: this thread's own store of the first pass)
-        const V y[1] = {value(d, to_f(kNorm ? xio[d] : src[d]))};
-        uint32_t b[1];
-        quantize<V, 1>(y, z, b);
-        q[d] = (int8_t)(b[0] & 0xffu);
-    }
+    for (int64_t d = threadIdx.x; d < a.dim; d += blockDim.x) // (with ADD: this thread's own stores of the first pass)
+        q[d] = (int8_t)(quantize1<kShort<T, SRC>>(value(d, to_f(kNorm ? xio[d] : src[d])), z) & 0xffu);
     if (threadIdx.x == 0)
         a.scales[row] = z.scale;
 }
 
-template <typename T, int SRC, int NV>
-int launch_rows_nv(const RowArgs &a, int64_t groups, cudaStream_t stream)
+constexpr int64_t kSmemPerSM = 220 * 1024;
+
+// CTAs of `threads` threads that an SM's registers hold (allocated in units of
+// 256 for a warp).
+template <typename T, int SRC, int NV, bool RAGGED, int THREADS>
+int stream_resident(int threads)
 {
-    const int threads = (int)(ceil_div(ceil_div(groups, NV), 32) * 32);
-    rows_int8_kernel<T, SRC, NV><<<(unsigned)a.n_rows, threads, 0, stream>>>(a);
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, rows_int8_stream_kernel<T, SRC, NV, RAGGED, THREADS>) == cudaSuccess ? f.numRegs
+                                                                                                              : 128;
+    }();
+    return std::max(1, 65536 / ((regs * 32 + 255) / 256 * 256 * (threads / 32)));
+}
+
+// The stream kernel on as many CTAs as an SM holds, with a ring that keeps about
+// 96 KB an SM in flight (64 to 128 KB measured the same within 2 %, 200 KB up to
+// 15 % slower) and at least two rows of each CTA where they fit.
+template <typename T, int SRC, int NV, bool RAGGED, int THREADS>
+int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes, cudaStream_t stream)
+{
+    auto kernel = rows_int8_stream_kernel<T, SRC, NV, RAGGED, THREADS>;
+    const int threads = (int)(ceil_div(ceil_div(a.dim, 8 * NV), 32) * 32);
+    const int64_t resident = std::min(16, stream_resident<T, SRC, NV, RAGGED, THREADS>(threads));
+    const int64_t per_sm = std::max<int64_t>(1, std::min(resident, kSmemPerSM / (2 * stage_bytes)));
+    const int64_t fits = kSmemPerSM / (per_sm * stage_bytes); // at least 1 (stage_bytes <= kSmemPerSM)
+    const int depth = (int)std::min({std::max<int64_t>(96 * 1024 / (per_sm * stage_bytes), 2), fits, (int64_t)kMaxDepth});
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemPerSM);
+    if (e != cudaSuccess)
+        return set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
+    const int64_t grid = std::min<int64_t>(a.n_rows, per_sm * num_sms());
+    kernel<<<(unsigned)grid, threads, (size_t)(depth * stage_bytes), stream>>>(a, depth, (uint32_t)input_bytes);
     return L2K_OK;
+}
+
+// Groups per thread: one for the shortest rows (a warp or less); four for 16-bit
+// rows (the reduction's fixed cost of about 60 instructions a warp is shared by
+// four groups: 16384 x 4096 bf16 rows 40 us, 44 with two), two where a few rows per
+// SM leave threads idle (512 rows: 4.0 us, 4.7 with one); two for fp32 rows (53 us,
+// 60 with four) and one for fp32 SwiGLU (90 us, 99 with two) and a few ragged
+// rows; more where the row needs it. SwiGLU rows of 416 to 448 threads would leave
+// an SM one CTA at their 77 registers: 4099 x 13824 f16 75 us, 61 with two.
+template <typename T, int SRC, bool RAGGED>
+int launch_stream(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes, cudaStream_t stream)
+{
+    constexpr bool kWide = sizeof(T) == 4, kNorm = SRC == SRC_NORM || SRC == SRC_NORM_ADD;
+    const int64_t groups = ceil_div(a.dim, 8);
+    const bool few = a.n_rows <= 4 * num_sms();
+    const int want = groups <= 32 || (kWide && SRC == SRC_SWIGLU) || (RAGGED && few) ? 1
+                     : kWide || groups <= 64 || (few && !kNorm)                      ? 2
+                                                                                     : 4;
+    if (want == 1 && groups <= kStreamThreads)
+        return launch_stream_nv<T, SRC, 1, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
+    if (want <= 2 && groups <= 2 * kStreamThreads)
+        return launch_stream_nv<T, SRC, 2, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
+    if constexpr (!kWide && SRC == SRC_SWIGLU && !RAGGED)
+        if (groups > 4 * 384 && groups <= 4 * kTwoPerSM)
+            return launch_stream_nv<T, SRC, 4, RAGGED, kTwoPerSM>(a, input_bytes, stage_bytes, stream);
+    return launch_stream_nv<T, SRC, 4, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
 }
 
 template <typename T, int SRC>
@@ -368,17 +884,26 @@ int launch_rows(const RowArgs &a, const char *name, cudaStream_t stream)
 {
     const bool vec = a.dim % 8 == 0 && is_aligned(a.x, 16) && is_aligned(a.xio, 16) && is_aligned(a.residual, 16) &&
                      is_aligned(a.w, 16) && is_aligned(a.q, 8);
-    const int64_t groups = a.dim / 8;
-    if (vec && groups <= kMaxThreads)
-        launch_rows_nv<T, SRC, 1>(a, groups, stream);
-    else if (vec && groups <= 2 * kMaxThreads)
-        launch_rows_nv<T, SRC, 2>(a, groups, stream);
-    else
+    const int64_t groups = ceil_div(a.dim, 8);
+    const int64_t row_bytes = a.dim * (SRC == SRC_SWIGLU ? 2 : 1) * (int64_t)sizeof(T);
+    const int64_t input_bytes = vec ? row_bytes : (row_bytes + 30) / 16 * 16; // (the 16-byte units a row touches)
+    const int64_t stage_bytes = input_bytes * (SRC == SRC_NORM_ADD ? 2 : 1);
+    const bool stream_fits = groups <= 4 * kStreamThreads && stage_bytes <= kSmemPerSM;
+    int st = L2K_OK;
+    if (vec && a.n_rows <= 2 * num_sms() && groups <= 2 * kMaxThreads)
     {
-        const int threads = (int)std::min<int64_t>(kMaxThreads, ceil_div(a.dim, 32) * 32);
-        rows_int8_any_kernel<T, SRC><<<(unsigned)a.n_rows, threads, 0, stream>>>(a);
+        // few rows: latency, so as many threads as there are groups
+        if (groups <= kMaxThreads)
+            rows_int8_kernel<T, SRC, 1><<<(unsigned)a.n_rows, (unsigned)(ceil_div(groups, 32) * 32), 0, stream>>>(a);
+        else
+            rows_int8_kernel<T, SRC, 2><<<(unsigned)a.n_rows, (unsigned)(ceil_div(groups, 64) * 32), 0, stream>>>(a);
     }
-    return check_launch(name);
+    else if (stream_fits)
+        st = vec ? launch_stream<T, SRC, false>(a, input_bytes, stage_bytes, stream)
+                 : launch_stream<T, SRC, true>(a, input_bytes, stage_bytes, stream);
+    else
+        rows_int8_any_kernel<T, SRC><<<(unsigned)a.n_rows, kMaxThreads, 0, stream>>>(a);
+    return st != L2K_OK ? st : check_launch(name);
 }
 
 // Checks common to the three entries; returns L2K_OK with *done set when
@@ -402,6 +927,21 @@ int check_rows(const RowArgs &a, int dtype, const char *name, cudaStream_t strea
 }
 
 } // namespace
+
+int read_int8_rows_error(bool clear)
+{
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_int8_rows_error, sizeof(int)) != cudaSuccess)
+        return -1;
+    if (clear && v)
+    {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(g_int8_rows_error, &zero, sizeof(int)) != cudaSuccess)
+            return -1;
+    }
+    return v;
+}
+
 } // namespace l2k
 
 extern "C" int l2k_quantize_rows_int8(const void *x, int8_t *q, float *scales, int64_t num_rows, int64_t dim,

@@ -553,6 +553,7 @@ int read_step_error(bool clear);   // decode_step.cu
 int read_pv_error(bool clear);     // attention_qkv_tc.cu
 int read_gemm_error(bool clear);   // gemm_tc.cu
 int read_int8_error(bool clear);   // gemm_int8_tc.cu
+int read_int8_rows_error(bool clear); // int8_rows.cu
 int read_gemv_error(bool clear);   // gemv.cu
 
 } // namespace l2k
@@ -575,9 +576,10 @@ extern "C" int l2k_device_error(int clear)
     const int v5 = l2k::read_gemm_error(clear != 0);
     const int v6 = l2k::read_gemv_error(clear != 0);
     const int v7 = l2k::read_int8_error(clear != 0);
-    if (v2 < 0 || v3 < 0 || v4 < 0 || v5 < 0 || v6 < 0 || v7 < 0)
+    const int v8 = l2k::read_int8_rows_error(clear != 0);
+    if (v2 < 0 || v3 < 0 || v4 < 0 || v5 < 0 || v6 < 0 || v7 < 0 || v8 < 0)
         return -1;
-    const int others[] = {v2, v3, v4, v5, v6, v7};
+    const int others[] = {v2, v3, v4, v5, v6, v7, v8};
     for (int o : others)
         if (!v && o)
             v = o;

@@ -1,6 +1,6 @@
 """Timings of single operators and of the decoder layer on one GPU.
 
-    python -m llama2_b200.microbench {gemm,attention,paged,paged_step,paged_prefill,fp8,pv,swiglu,unpad,rope,layer} [--iters N]
+    python -m llama2_b200.microbench {gemm,attention,paged,paged_step,paged_prefill,fp8,pv,swiglu,unpad,rope,layer,int8} [--iters N]
 
 Each prints one line per shape. Kernels are timed with CUDA events on the
 current stream; ``gemm`` times back-to-back launches of the products of
@@ -331,17 +331,60 @@ def bench_layer(iters):
         del layer
 
 
+def bench_int8(iters, shape=None):
+    """The 8-bit (W8A8) operators: the row operators in GB/s of their operands
+    and results, the products next to launch_linear on 16-bit operands of the
+    same sizes (in GB/s up to 128 rows, else in integer TOP/s)."""
+    for dt in (torch.bfloat16, torch.float32):
+        es = 2 if dt == torch.bfloat16 else 4
+        for (n, d) in ([] if shape else [(1, 4096), (64, 4096), (64, 5120), (16384, 4096), (16384, 11008), (333, 1023)]):
+            x = torch.randn(n, d, device="cuda").to(dt)
+            r = torch.zeros(n, d, device="cuda", dtype=dt)
+            gu = torch.randn(n, 2 * d, device="cuda").to(dt)
+            w = torch.ones(d, device="cuda", dtype=dt)
+            q = torch.empty(n, d, dtype=torch.int8, device="cuda")
+            s = torch.empty(n, device="cuda")
+            for name, fn, nb in (
+                    ("rows", lambda: ops.launch_quantize_rows_int8(x, q, s), es + 1),
+                    ("add-residual RMSNorm", lambda: ops.launch_fused_add_residual_rmsnorm_int8(w, x, r, q, s, True),
+                     3 * es + 1),
+                    ("SwiGLU", lambda: ops.launch_swiglu_int8(gu, q, s), 2 * es + 1)):
+                t = time_ms(fn, iters)
+                print(f"int8 {name} {dt} {n} x {d}: {t * 1e3:.1f} us {nb * n * d / t / 1e6:.1f} GB/s")
+    for (m, n, k) in ([shape] if shape else [
+            (1, 4096, 4096), (1, 12288, 4096), (1, 22016, 4096), (1, 4096, 11008), (64, 4096, 4096), (64, 12288, 4096),
+            (64, 22016, 4096), (64, 4096, 11008), (128, 12288, 4096), (200, 4096, 4096), (257, 1003, 2064),
+            (512, 12288, 4096), (1024, 4096, 4096), (2048, 12288, 4096), (16384, 4096, 4096), (16384, 12288, 4096),
+            (16384, 22016, 4096), (16384, 4096, 11008)]):
+        a = torch.randint(-127, 128, (m, k), device="cuda", dtype=torch.int8)
+        b = torch.randint(-127, 128, (n, k), device="cuda", dtype=torch.int8)
+        sa, sb = torch.ones(m, device="cuda"), torch.ones(n, device="cuda")
+        c = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+        flush = m <= 1024
+        t = time_ms(lambda: ops.launch_linear_int8(a, sa, b, sb, c), iters, flush=flush)
+        a16, b16 = a.to(torch.bfloat16), b.to(torch.bfloat16)
+        t16 = time_ms(lambda: ops.launch_linear(False, True, m, n, k, a16, b16, c), iters, flush=flush)
+        if m <= 128:
+            rate = f"{(m * k + n * k + 2 * m * n) / t / 1e6:.1f} GB/s"
+        else:
+            rate = f"{2.0 * m * n * k / t / 1e9:.1f} TOP/s"
+        print(f"int8 product m={m} n={n} k={k}{' (L2 flushed)' if flush else ''}: {t * 1e3:.1f} us {rate} | "
+              f"bf16 {t16 * 1e3:.1f} us")
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("what", choices=["gemm", "attention", "paged", "paged_step", "paged_prefill", "fp8", "pv", "swiglu", "unpad",
-                                        "rope", "layer"])
+                                        "rope", "layer", "int8"])
     ap.add_argument("--iters", type=int, default=20)
-    ap.add_argument("--shape", default="", help="gemm: one M,N,K product (B stored K x N) instead of the set")
+    ap.add_argument("--shape", default="", help="gemm, int8: one M,N,K product instead of the set (gemm: B stored K x N)")
     ap.add_argument("--batch", type=int, default=0, help="fp8: one batch size instead of the set")
     args = ap.parse_args()
     torch.manual_seed(0)
     if args.what == "gemm":
         bench_gemm(args.iters, tuple(int(x) for x in args.shape.split(",")) if args.shape else None)
+    elif args.what == "int8":
+        bench_int8(args.iters, tuple(int(x) for x in args.shape.split(",")) if args.shape else None)
     elif args.what == "fp8":
         bench_fp8(args.iters, args.batch or None)
     else:

@@ -571,18 +571,36 @@ def prefill_attention_scores(q, k, q_lens, kv_lens, max_q_len, max_kv_len, qk):
 # --------------------------------------------------------------------------
 def _int8_rows(q, scales, n, dim, name):
     """Checks an int8 row tensor (n, dim) and its scales (n)."""
-    _require(q.dtype == torch.int8, f"{name} must be an int8 tensor, got {q.dtype}")
-    _require(scales.dtype == torch.float32, f"the scales of {name} must be float32, got {scales.dtype}")
-    _require(tuple(q.shape) == (n, dim), f"Incorrect {name} size")
-    _require(tuple(scales.shape) == (n,), f"Incorrect size of the scales of {name}")
+    if q.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise ValueError(f"{name} must be an int8 tensor with float32 scales, got {q.dtype} and {scales.dtype}")
+    if q.shape != (n, dim):
+        raise ValueError(f"Incorrect {name} size")
+    if scales.shape != (n,):
+        raise ValueError(f"Incorrect size of the scales of {name}")
 
 
-def _one_device(*ts):
-    """The CUDA device that all the tensors are on, made current for the call."""
-    for t in ts[1:]:
-        if t.device != ts[0].device:
+def _one_device(*ts) -> int:
+    """The CUDA device that all the tensors are on."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != dev:
             raise ValueError(f"tensors are on different devices: {ts[0].device} and {t.device}")
-    return torch.cuda.device(ts[0].device)
+    return dev
+
+
+def _call_on(dev, name, *args):
+    """The entry point on device `dev` and its current stream (not the current
+    device's, where that is another one)."""
+    if dev == torch.cuda.current_device():
+        capi.call(name, *args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            capi.call(name, *args, _raw_stream(dev))
+
+
+def _raw_stream(dev) -> int:
+    """torch.cuda.current_stream(dev).cuda_stream without the stream object (3 us)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def launch_quantize_rows_int8(x, q, scales):
@@ -591,37 +609,39 @@ def launch_quantize_rows_int8(x, q, scales):
     _dev(x, q, scales)
     n, dim = x.shape
     _int8_rows(q, scales, n, dim, "q")
-    with _one_device(x, q, scales):
-        capi.call("l2k_quantize_rows_int8", x.data_ptr(), q.data_ptr(), scales.data_ptr(), n, dim, _code(x), _stream())
+    _call_on(_one_device(x, q, scales), "l2k_quantize_rows_int8", x.data_ptr(), q.data_ptr(), scales.data_ptr(), n,
+             dim, _code(x))
 
 
 def launch_fused_add_residual_rmsnorm_int8(weights, x, residual, q, scales, add_residual: bool):
     """launch_fused_add_residual_rmsnorm with the normed rows as int8 (q, scales):
     x is updated in place with add_residual; residual is read only (None
     without add_residual)."""
-    ts = (weights, x, q, scales) + ((residual,) if add_residual else ())
+    ts = (weights, x, q, scales, residual) if add_residual else (weights, x, q, scales)
     _dev(*ts)
     _same(x, weights, "launch_fused_add_residual_rmsnorm_int8")
     n, dim = x.shape
     if add_residual:
         _same(x, residual, "launch_fused_add_residual_rmsnorm_int8")
-        _require(tuple(residual.shape) == (n, dim), "Incorrect residual size")
-    _require(tuple(weights.shape) == (dim,), "Incorrect rmsnorm weight size")
+        if residual.shape != (n, dim):
+            raise ValueError("Incorrect residual size")
+    if weights.shape != (dim,):
+        raise ValueError("Incorrect rmsnorm weight size")
     _int8_rows(q, scales, n, dim, "q")
-    with _one_device(*ts):
-        capi.call("l2k_fused_add_residual_rmsnorm_int8", weights.data_ptr(), x.data_ptr(),
-                  residual.data_ptr() if add_residual else None, q.data_ptr(), scales.data_ptr(), n, dim,
-                  int(bool(add_residual)), _code(x), _stream())
+    _call_on(_one_device(*ts), "l2k_fused_add_residual_rmsnorm_int8", weights.data_ptr(), x.data_ptr(),
+             residual.data_ptr() if add_residual else None, q.data_ptr(), scales.data_ptr(), n, dim,
+             int(bool(add_residual)), _code(x))
 
 
 def launch_swiglu_int8(input, q, scales):
     """launch_swiglu with the output rows as int8: input (N, 2F) -> q (N, F), scales (N,)."""
     _dev(input, q, scales)
     n, f = q.shape
-    _require(tuple(input.shape) == (n, 2 * f), "Incorrect input size")
+    if input.shape != (n, 2 * f):
+        raise ValueError("Incorrect input size")
     _int8_rows(q, scales, n, f, "q")
-    with _one_device(input, q, scales):
-        capi.call("l2k_swiglu_int8", input.data_ptr(), q.data_ptr(), scales.data_ptr(), n, f, _code(input), _stream())
+    _call_on(_one_device(input, q, scales), "l2k_swiglu_int8", input.data_ptr(), q.data_ptr(), scales.data_ptr(), n, f,
+             _code(input))
 
 
 def launch_linear_int8(A, a_scales, B, b_scales, C):
@@ -629,15 +649,14 @@ def launch_linear_int8(A, a_scales, B, b_scales, C):
     with a scale per token, B (N, K) (a weight [out, in]) with a scale per output
     channel, C (M, N) float32, float16 or bfloat16; exact integer sums."""
     _dev(A, a_scales, B, b_scales, C)
-    _require(A.dim() == 2 and B.dim() == 2 and C.dim() == 2, "Matrix dim do not match")
     m, k = A.shape
-    n = B.shape[0]
+    n, kb = B.shape
     _int8_rows(A, a_scales, m, k, "A")
-    _int8_rows(B, b_scales, n, k, "B")
-    _require(tuple(C.shape) == (m, n), "Incorrect C size")
-    with _one_device(A, a_scales, B, b_scales, C):
-        capi.call("l2k_linear_int8", m, n, k, A.data_ptr(), k, a_scales.data_ptr(), B.data_ptr(), k,
-                  b_scales.data_ptr(), C.data_ptr(), n, _code(C), _stream())
+    _int8_rows(B, b_scales, n, kb, "B")
+    if kb != k or C.shape != (m, n):
+        raise ValueError("Matrix sizes do not match")
+    _call_on(_one_device(A, a_scales, B, b_scales, C), "l2k_linear_int8", m, n, k, A.data_ptr(), k,
+             a_scales.data_ptr(), B.data_ptr(), k, b_scales.data_ptr(), C.data_ptr(), n, _code(C))
 
 
 # --------------------------------------------------------------------------

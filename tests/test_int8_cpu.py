@@ -1,8 +1,6 @@
 """Refusals of the 8-bit (W8A8) operators, before anything is launched: at the
 C ABI (bad sizes, types, null pointers) and in llama2_b200.ops (types, shapes,
 devices of the tensors)."""
-import contextlib
-
 import pytest
 import torch
 
@@ -61,12 +59,21 @@ def test_empty_inputs_are_noops():
 @pytest.fixture
 def host_tensors(monkeypatch):
     """The operators' checks on host tensors: the device check passes, a launch fails the test."""
-    def call(name, *args):
+    def call(dev, name, *args):
         raise AssertionError(f"{name} was launched")
 
     monkeypatch.setattr(ops, "_dev", lambda *ts: None)
-    monkeypatch.setattr(ops, "_one_device", lambda *ts: contextlib.nullcontext())
-    monkeypatch.setattr(capi, "call", call)
+    monkeypatch.setattr(ops, "_call_on", call)
+
+
+class OnDevice:
+    """What _one_device asks of a tensor."""
+
+    def __init__(self, dev):
+        self.device = f"cuda:{dev}"
+
+    def get_device(self):
+        return int(self.device[-1])
 
 
 def i8(*s):
@@ -101,8 +108,33 @@ def test_ops_refuse(host_tensors, fn):
         fn()
 
 
+def test_launch_on_the_tensors_device(monkeypatch):
+    """The device of the tensors is current during the call, its current stream
+    is used, and the caller's device is restored."""
+    calls, current = [], [0]
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.old, current[0] = current[0], self.dev
+
+        def __exit__(self, *a):
+            current[0] = self.old
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 100 + dev)
+    monkeypatch.setattr(capi, "call", lambda name, *args: calls.append((current[0], name, *args)))
+    ops._call_on(0, "f", 1)
+    ops._call_on(1, "f", 2)
+    assert calls == [(0, "f", 1, 100), (1, "f", 2, 101)] and current[0] == 0
+
+
 def test_host_tensors_and_mixed_devices_are_refused():
     with pytest.raises(ValueError, match="CUDA device"):
         ops.launch_quantize_rows_int8(f32(3, 8), i8(3, 8), f32(3))
     with pytest.raises(ValueError, match="different devices"):
-        ops._one_device(f32(3), torch.empty(3, device="meta"))
+        ops._one_device(OnDevice(0), OnDevice(0), OnDevice(1))
+    assert ops._one_device(OnDevice(1), OnDevice(1)) == 1

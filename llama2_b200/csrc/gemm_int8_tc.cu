@@ -159,6 +159,34 @@ __device__ __forceinline__ void store8(T *out, const uint32_t *r, float row_scal
     }
 }
 
+// 32 consecutive columns of this lane's row, from their integer sums, into row
+// `lane` of a 128-byte-swizzled staging tile, from its column c on. sb: the b_scale
+// of the lane-th of these columns.
+template <typename T>
+__device__ __forceinline__ void scale_to_rows(const uint32_t (&r)[32], float row_scale, float sb, uint8_t *staging, int lane,
+                                              int c)
+{
+    constexpr int N = Vec16<T>::N;
+#pragma unroll
+    for (int v = 0; v < 32 / N; ++v)
+    {
+        Vec16<T> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            o.v[e] = from_f<T>(__fmul_rn((float)(int)r[N * v + e],
+                                         __fmul_rn(row_scale, __shfl_sync(0xffffffffu, sb, N * v + e))));
+        const int unit = (c / N + v) ^ (lane & 7); // the 16-byte units of a row, permuted by the row
+        *reinterpret_cast<uint4 *>(staging + 128 * lane + 16 * unit) = as_u4(o);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T staged(const uint8_t *staging, int row, int col)
+{
+    constexpr int N = Vec16<T>::N;
+    return *reinterpret_cast<const T *>(staging + 128 * row + 16 * ((col / N) ^ (row & 7)) + sizeof(T) * (col % N));
+}
+
 // ---------------------------------------------------------------------------
 // One BM x bn tile per cluster of `split` CTAs, each a K range. Within a CTA the
 // k blocks are dealt to `groups` (1, 2 or 4) of one producer and one MMA warp
@@ -168,7 +196,8 @@ __device__ __forceinline__ void store8(T *out, const uint32_t *r, float row_scal
 // issues its first loads at once, before tensor memory is allocated. The
 // epilogue adds the accumulators; integer sums do not depend on the dealing.
 //
-// split > 1: every rank leaves its partial tile in its own shared memory (the
+// split > 1 (or rows of C without 16-byte alignment, whose stores should be to
+// neighbours): every rank leaves its partial tile in its own shared memory (the
 // drained ring). After a cluster barrier each rank adds its rows [q rows_per,
 // (q + 1) rows_per) into rank q's copy with one bulk reduction, and rank q
 // scales and stores those rows once all have landed. A last barrier keeps every
@@ -191,14 +220,14 @@ struct TileShape
     uint32_t stage_bytes, ring_bytes, smem_bytes;
     int a_rows;
 };
-inline TileShape tile_shape(int64_t m, int bm, int bn, int split, int groups)
+inline TileShape tile_shape(int64_t m, int bm, int bn, int split, int groups, bool stage)
 {
     TileShape t{bm, bn, split, groups, 0, 0, 0, 0, 0};
     t.a_rows = (int)std::min<int64_t>(bm, ceil_div(m, 8) * 8);
     t.stage_bytes = (uint32_t)(bn + t.a_rows) * 128;
     const uint32_t slack = (uint32_t)(bm - t.a_rows) * 128; // what the last stage's MMAs read past its A rows
     t.stages = (int)std::min<uint32_t>(kTMaxStages, (kTRing - slack) / t.stage_bytes) / groups * groups;
-    const uint32_t staged = split > 1 ? (uint32_t)bm * (bn + 4) * 4 : 0;
+    const uint32_t staged = stage ? (uint32_t)bm * (bn + 4) * 4 : 0;
     t.ring_bytes = (std::max(t.stages * t.stage_bytes + slack, staged) + 1023) & ~1023u;
     t.smem_bytes = t.ring_bytes + 4 * (uint32_t)bn + 8 * (2 * kTMaxStages + 2) + 16;
     return t;
@@ -401,7 +430,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 r[e] += x[e];
         }
     };
-    if (split == 1)
+    if (split == 1 && a.wide)
     {
         T *out = static_cast<T *>(a.c) + (row0 + lrow) * a.ldc + col0;
 #pragma unroll 1
@@ -413,7 +442,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
             {
 #pragma unroll
                 for (int v = 0; v < 32; v += 8)
-                    store8<T>(out + c0 + v, r + v, row_scale, sb + c0 + v, a.n - col0 - c0 - v, a.wide);
+                    store8<T>(out + c0 + v, r + v, row_scale, sb + c0 + v, a.n - col0 - c0 - v, true);
             }
             __syncwarp();
         }
@@ -499,8 +528,8 @@ constexpr int kPThreads = 64 + 256;                 // producer warp, MMA warp, 
 constexpr int kPStages = 6;
 constexpr uint32_t kPHalf = 128 * 128;              // one CTA's half of an operand: 128 rows x 128 k
 constexpr uint32_t kPStageBytes = 2 * kPHalf;
-constexpr uint32_t kPOffScales = kPStages * kPStageBytes; // 128 b_scales per epilogue warp
-constexpr uint32_t kPOffBar = kPOffScales + 8 * 128 * 4;
+constexpr uint32_t kPOffOut = kPStages * kPStageBytes;    // 32 rows x 128 bytes of C per epilogue warp
+constexpr uint32_t kPOffBar = kPOffOut + 8 * 4096;
 constexpr uint32_t kPOffMisc = kPOffBar + 8 * (2 * kPStages + 4);
 constexpr uint32_t kPSmemBytes = kPOffMisc + 16;
 
@@ -525,10 +554,25 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster)
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
+// The tile's row and column of tiles: bands of 16 columns, each walked row by row,
+// so that the tiles in flight (74 on B200) share 16 tiles of B and about 5 of A in
+// L2 (row by row over all columns: 8192 x 27648 x 5120 885 us, 743 in bands).
+constexpr int64_t kPBand = 16;
+struct TileAt
+{
+    int64_t row, col;
+};
+__device__ __forceinline__ TileAt tile_at(int64_t tile, int64_t m_tiles, int64_t n_tiles)
+{
+    const int64_t band = tile / (m_tiles * kPBand), rest = tile - band * m_tiles * kPBand;
+    const int64_t width = n_tiles - band * kPBand < kPBand ? n_tiles - band * kPBand : kPBand;
+    return TileAt{rest / width, band * kPBand + rest % width};
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kPThreads, 1)
     linear_int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                            const __grid_constant__ Int8Args a)
+                            const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ Int8Args a)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -544,7 +588,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0); // (uniform, known as such)
-    const int64_t n_tiles = ceil_div_dev(a.m, 256) * a.n_nt;
+    const int64_t m_tiles = ceil_div_dev(a.m, 256), n_tiles = m_tiles * a.n_nt;
     const int64_t cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
     const int n_kb = a.n_kb;
     const bool misaligned = (sbase & 1023u) != 0; // uniform over the cluster (same layout); acted on after the sync
@@ -588,8 +632,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
         uint32_t phase = 1; // (a fresh barrier's previous phase counts as complete)
         for (int64_t tile = cluster_id; tile < n_tiles && !misaligned; tile += n_clusters)
         {
-            const int row0 = (int)(tile / a.n_nt) * 256 + 128 * (int)rank;
-            const int col0 = (int)(tile % a.n_nt) * 256 + 128 * (int)rank;
+            const TileAt t = tile_at(tile, m_tiles, a.n_nt);
+            const int row0 = (int)t.row * 256 + 128 * (int)rank, col0 = (int)t.col * 256 + 128 * (int)rank;
             int kb = 0;
             for (; kb < n_kb; ++kb)
             {
@@ -674,19 +718,19 @@ __global__ void __launch_bounds__(kPThreads, 1)
         // epilogue warps 2..: TMEM lane quadrant warp % 4 holds rows 32 (warp % 4) + lane of this CTA's half;
         // the two warps of a quadrant share its columns
         const int quad = warp & 3, part = (warp - 2) >> 2;
-        float *sb = reinterpret_cast<float *>(smem + kPOffScales) + 128 * (warp - 2); // this warp's 128 columns
+        uint8_t *staging = smem + kPOffOut + 4096 * (warp - 2);
         int64_t lt = 0;
         for (int64_t tile = cluster_id; tile < n_tiles && !*abort_flag; tile += n_clusters, ++lt)
         {
             const int buf = (int)(lt & 1);
-            const int64_t row = (tile / a.n_nt) * 256 + 128 * (int64_t)rank + 32 * quad + lane;
-            const int64_t col0 = (tile % a.n_nt) * 256 + 128 * part;
+            const TileAt t = tile_at(tile, m_tiles, a.n_nt);
+            const int64_t row = t.row * 256 + 128 * (int64_t)rank + 32 * quad + lane, col0 = t.col * 256 + 128 * part;
             const bool store = row < a.m;
             const float row_scale = store ? __ldg(a.sa + row) : 0.f;
+            float sb[4]; // the scales of this warp's columns 32 i + lane
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                sb[32 * i + lane] = col0 + 32 * i + lane < a.n ? __ldg(a.sb + col0 + 32 * i + lane) : 0.f;
-            __syncwarp();
+                sb[i] = col0 + 32 * i + lane < a.n ? __ldg(a.sb + col0 + 32 * i + lane) : 0.f;
             if (!mbar_wait(bar_acc_full + 8 * buf, (uint32_t)(lt >> 1) & 1u, abort_flag))
             {
                 int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
@@ -695,26 +739,58 @@ __global__ void __launch_bounds__(kPThreads, 1)
             __syncwarp();
             tc_fence_after();
             const uint32_t taddr = tmem + (uint32_t)(buf * 256 + 128 * part) + ((uint32_t)(32 * quad) << 16);
-            T *out = static_cast<T *>(a.c) + row * a.ldc + col0;
-#pragma unroll 1
-            for (int c0 = 0; c0 < 128; c0 += 32)
+            if (a.wide)
             {
-                uint32_t r[32];
-                tmem_ld32_async(taddr + (uint32_t)c0, r);
-                tmem_wait_ld();
-                if (store)
-                {
+                // through shared memory (128-byte swizzle) and TMA, 32 rows x 128 bytes at a time:
+                // whole lines, where each lane's own 16-byte stores touch 32 lines per instruction
+                constexpr int kCols = 128 / (int)sizeof(T); // columns per store: 64 or 32
 #pragma unroll
-                    for (int v = 0; v < 32; v += 8)
-                        store8<T>(out + c0 + v, r + v, row_scale, sb + c0 + v, a.n - col0 - c0 - v, a.wide);
+                for (int c0 = 0; c0 < 128; c0 += kCols)
+                {
+                    bulk_wait_read_0(); // the previous store has read the staging rows
+                    __syncwarp();
+#pragma unroll
+                    for (int h = 0; h < kCols; h += 32)
+                    {
+                        uint32_t r[32];
+                        tmem_ld32_async(taddr + (uint32_t)(c0 + h), r);
+                        tmem_wait_ld();
+                        scale_to_rows<T>(r, row_scale, sb[(c0 + h) / 32], staging, lane, h);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (col0 + c0 < a.n && elect_one())
+                        tma_store_3d(&tm_c, smem_u32(staging), (int)(col0 + c0), (int)(row - lane), 0);
+                    bulk_commit(); // (an empty group in the other lanes)
                 }
-                __syncwarp();
+            }
+            else
+            {
+                // rows of no 16-byte alignment: staged the same way, then a row at a time, a warp's
+                // lanes storing neighbouring elements
+                const int64_t rows = a.m - (row - lane);
+                T *out = static_cast<T *>(a.c) + (row - lane) * a.ldc + col0;
+#pragma unroll
+                for (int c0 = 0; c0 < 128; c0 += 32)
+                {
+                    uint32_t r[32];
+                    tmem_ld32_async(taddr + (uint32_t)c0, r);
+                    tmem_wait_ld();
+                    scale_to_rows<T>(r, row_scale, sb[c0 / 32], staging, lane, 0);
+                    __syncwarp();
+                    const bool in = col0 + c0 + lane < a.n;
+                    for (int i = 0; i < 32 && i < rows; ++i)
+                        if (in)
+                            out[i * a.ldc + c0 + lane] = staged<T>(staging, i, lane);
+                    __syncwarp();
+                }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
                 mbar_arrive_cluster(acc_empty0 + 8 * buf);
         }
+        bulk_wait_read_0(); // the last stores have read their rows
     }
 
     // -------- teardown: after a failure, copies and MMAs in flight land first --------
@@ -823,7 +899,7 @@ int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
 {
     while (groups > 1 && (groups * bn > 512 || groups > a.n_kb / split)) // 512 TMEM columns, a k block for each
         groups /= 2;
-    const TileShape t = tile_shape(a.m, BM, bn, split, groups);
+    const TileShape t = tile_shape(a.m, BM, bn, split, groups, split > 1 || !a.wide);
     a.bn = bn;
     a.split = split;
     a.kb_per = a.n_kb / split;
@@ -871,6 +947,16 @@ int launch_pair(Int8Args a, cudaStream_t stream)
     if (!make_map(&ma, dt, a.a, k, m, 1, lda, lda * m, 128, kBK) ||
         !make_map(&mb, dt, a.b, k, n, 1, ldb, ldb * n, 128, kBK))
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
+    CUtensorMap mc = {};
+    if (a.wide)
+    {
+        const CUtensorMapDataType ct = std::is_same<T, float>::value   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const uint64_t ldc_bytes = (uint64_t)a.ldc * sizeof(T);
+        if (!make_map(&mc, ct, a.c, n, m, 1, ldc_bytes, ldc_bytes * m, 32, 128 / sizeof(T)))
+            return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
+    }
     auto kernel = linear_int8_pair_kernel<T>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmemBytes);
     if (e != cudaSuccess)
@@ -888,54 +974,130 @@ int launch_pair(Int8Args a, cudaStream_t stream)
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
+    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, a);
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8 (two-SM tiles): %s", cudaGetErrorString(e));
     return check_launch("l2k_linear_int8 (two-SM tiles)");
 }
 
-// Which kernel, and its tiles: the least estimated time, in clocks of an SM at
-// 1.9 GHz, from rates measured with these kernels on B200. A k block of a tile
-// takes the longest of its MMAs (bn / 2 each, for 64 and for 128 rows), its
-// issue (380 per warp) and its bytes at 56 per clock from L2; the whole product
-// at least its bytes at 3400 per clock from HBM. On top of that: 5000 for launch,
-// first loads and last stores, 3000 more for a reduction over a cluster, 18000 in
-// place of both for the two-SM kernel (whose tiles cover 2 SMs and end with 128
-// columns per warp to store).
+// Which kernel, and its tiles.
 struct Plan
 {
     int bm, bn, split, groups; // bm 256: the two-SM kernel
 };
-Plan plan(int64_t m, int64_t n, int n_kb)
+
+// Clusters of `split` CTAs of the tile kernel that the device runs at once (one CTA
+// per SM; cached per device).
+template <typename T>
+int resident_clusters(int split)
 {
-    const int64_t sms = num_sms();
-    const double dram = ((double)m + n) * n_kb * kBK / 3400.0 + 2.0 * m * n / 3400.0;
+    static std::mutex mu;
+    static int cache[64][9] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+        return 1;
+    std::lock_guard<std::mutex> lock(mu);
+    int &c = cache[dev][split];
+    if (c == 0)
+    {
+        auto kernel = linear_int8_tile_kernel<T, 128>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)split);
+        cfg.blockDim = dim3(kTThreads);
+        cfg.dynamicSmemBytes = kTRing;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)split;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTMaxSmem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess)
+            (void)cudaGetLastError();
+        c = n > 0 ? n : 1;
+    }
+    return c;
+}
+
+// The least estimated time, in SM clocks. The estimate was fitted to 2 900 timings
+// (165 sizes of 1 to 3000 rows, 300 to 32000 columns and 512 to 13824 k, under
+// every tile, split and group count): its choice takes 0.9 % longer than the best
+// of each size on the average, 16 % at worst. A tile's k block takes the longest
+// of its MMAs (2 bn), its issue (450 shared by the groups) and its bytes at 79 per
+// clock from L2; a wave of tiles ends with its last stores (15.5 bn, and 2.2 bn for
+// each further accumulator); the product takes at least its bytes at 3657 per clock
+// from HBM, and 0.62 of the shorter of the two on top of the longer; then 5300 for
+// launch, first loads and teardown, and for the reduction over a cluster 740 and a
+// quarter of the tile's elements. The two-SM kernel: 438 a k block, 11000 once.
+template <typename T>
+Plan estimate(int64_t m, int64_t n, int n_kb)
+{
+    const int64_t pairs = num_sms() / 2;
+    const double dram = ((double)(m + n) * n_kb * kBK + 2.0 * m * n) / 3657.0;
+    auto together = [&](double run) { return std::max(run, dram) + 0.62 * std::min(run, dram); };
     Plan best{256, 256, 1, 1};
-    double best_t = std::max(dram, (double)ceil_div(ceil_div(m, 256) * ceil_div(n, 256), sms / 2) * n_kb * 585.0) + 18000.0;
+    double best_t = together((double)ceil_div(ceil_div(m, 256) * ceil_div(n, 256), pairs) * n_kb * 438.0) + 11040.0;
     const int bm = m <= 64 ? 64 : 128;
     const int64_t mt = ceil_div(m, bm), a_rows = std::min<int64_t>(bm, ceil_div(m, 8) * 8);
-    if (mt * ceil_div(n, 256) > 4 * sms || mt > 65535 || ceil_div(n, 32) > 65535)
-        return best;
+    if (mt > 65535 || ceil_div(n, 32) > 65535 || mt * ceil_div(n, 256) > 16 * pairs)
+        return best; // (many tiles: far in the two-SM kernel's range)
     for (int bn = 32; bn <= 256; bn += 32)
         for (int split = 1; split <= 8 && split <= n_kb; ++split)
         {
-            const int64_t ctas = mt * ceil_div(n, bn) * split;
-            if (split > 1 && ctas > sms)
-                break;
-            const int per = (int)ceil_div(n_kb, split);
-            int groups = bn <= 64 && bm == 64 ? 4 : 2;
-            while (groups > 1 && groups > n_kb / split)
-                groups /= 2;
-            const double kb = std::max({2.0 * bn, 380.0 / groups, (double)(bn + a_rows) * 128 / 56.0});
-            const double t = std::max(dram, (double)ceil_div(ctas, sms) * (per * kb + 10.0 * bn)) + 5000.0 +
-                             (split > 1 ? 3000.0 : 0.0);
-            if (t < best_t)
+            const int64_t tiles = mt * ceil_div(n, bn), resident = resident_clusters<T>(split);
+            if (split > 1 && tiles > resident)
+                break; // a second wave of split tiles
+            const double waves = (double)ceil_div(tiles, resident), per = (double)ceil_div(n_kb, split);
+            for (int groups = bn < 128 ? 2 : 1; groups <= (bn <= 96 ? 4 : 2); groups *= 2)
             {
-                best_t = t;
-                best = Plan{bm, bn, split, groups};
+                if (groups > 1 && groups > n_kb / split)
+                    continue;
+                const double kb = std::max({2.0 * bn, 450.0 / groups, (double)(bn + a_rows) * 128 / 79.0});
+                const double run = waves * (per * kb + (15.5 + 2.2 * (groups - 1)) * bn);
+                const double t = together(run) + 5337.0 + (split > 1 ? 737.0 + 0.255 * bm * bn : 0.0);
+                if (t < best_t)
+                {
+                    best_t = t;
+                    best = Plan{bm, bn, split, groups};
+                }
+            }
+            if (bn < 128 && n_kb / split < 2) // too few k blocks for two groups
+            {
+                const double run = waves * (per * 450.0 + 15.5 * bn);
+                const double t = together(run) + 5337.0 + (split > 1 ? 737.0 + 0.255 * bm * bn : 0.0);
+                if (t < best_t)
+                {
+                    best_t = t;
+                    best = Plan{bm, bn, split, 1};
+                }
             }
         }
     return best;
+}
+
+// estimate(), remembered for the sizes last asked for (a pure function of them and
+// the device's SM count).
+template <typename T>
+Plan plan(int64_t m, int64_t n, int n_kb)
+{
+    struct Entry
+    {
+        int64_t m = -1, n = 0;
+        int n_kb = 0;
+        Plan p{};
+    };
+    static thread_local Entry cache[64];
+    Entry &e = cache[(uint64_t)(m * 31 + n * 7 + n_kb) % 64];
+    if (e.m != m || e.n != n || e.n_kb != n_kb)
+    {
+        e.p = estimate<T>(m, n, n_kb);
+        e.m = m;
+        e.n = n;
+        e.n_kb = n_kb;
+    }
+    return e.p;
 }
 
 template <typename T>
@@ -948,7 +1110,7 @@ int launch_linear(const Int8Args &p, cudaStream_t stream)
                     encode_fn() != nullptr;
     if (!tc)
         return launch_any<T>(a, stream);
-    const Plan t = plan(a.m, a.n, a.n_kb);
+    const Plan t = plan<T>(a.m, a.n, a.n_kb);
     if (t.bm == 64)
         return launch_tile<T, 64>(a, t.bn, t.split, t.groups, stream);
     if (t.bm == 128)

@@ -30,6 +30,14 @@ tensor cores) the QKV projection takes the RoPE + K/V append into its
 epilogue and the gate/up projection the SwiGLU (``fuse_epilogues``, on by
 default): two launches fewer and neither product goes to HBM, with results
 bit-identical to the separate launches.
+
+``int8=True`` holds the four projections as 8-bit integers with one scale per
+output channel ([out, in] rows) and gives them 8-bit activations with one scale
+per token (W8A8): the norms and the SwiGLU write int8 rows
+(launch_fused_add_residual_rmsnorm_int8, launch_swiglu_int8), the attention
+output is quantised by launch_quantize_rows_int8, and the products are
+launch_linear_int8; residual stream, RoPE, caches and attention are those of the
+other layers, in ``dtype``. Ten launches per decode step, twelve per prefill.
 """
 from __future__ import annotations
 
@@ -40,16 +48,39 @@ import torch
 from . import ops
 
 
+class Int8Rows:
+    """Activations of one step as int8 rows: q (rows, dim) and scales (rows,)."""
+
+    def __init__(self, rows: int, dim: int, device):
+        self.q = torch.empty(rows, dim, dtype=torch.int8, device=device)
+        self.scales = torch.empty(rows, dtype=torch.float32, device=device)
+
+
+class Int8Weight(Int8Rows):
+    """A projection held for launch_linear_int8: q [out, in], one scale per
+    output channel, quantised from a [in, out] weight of a 16-bit or fp32 layer."""
+
+    def __init__(self, w: torch.Tensor):
+        super().__init__(w.shape[1], w.shape[0], w.device)
+        self.assign(w)
+
+    def assign(self, w: torch.Tensor):
+        """Takes the values of another [in, out] weight, in place."""
+        ops.launch_quantize_rows_int8(w.t().contiguous(), self.q, self.scales)
+
+
 class DecoderLayer:
     def __init__(self, dim: int, heads: int, kv_heads: int, hidden: int, kv_cache_len: int, batch: int,
-                 dtype=torch.bfloat16, device="cuda", seed: int = 0, pairing: int = 1, fuse_epilogues: bool = True):
+                 dtype=torch.bfloat16, device="cuda", seed: int = 0, pairing: int = 1, fuse_epilogues: bool = True,
+                 int8: bool = False):
         if dim % heads or heads % kv_heads:
             raise ValueError("dim must be a multiple of heads, heads of kv_heads")
         self.dim, self.heads, self.kv_heads, self.hidden = dim, heads, kv_heads, hidden
         self.head_dim = dim // heads
         self.kv_cache_len, self.batch, self.dtype, self.pairing = kv_cache_len, batch, dtype, pairing
         # the epilogue kernels' shape rules (16-bit, head_dim 64 or 128, F % 8 == 0)
-        self.fuse_epilogues = (fuse_epilogues and dtype != torch.float32 and self.head_dim in (64, 128)
+        self.int8 = int8
+        self.fuse_epilogues = (fuse_epilogues and not int8 and dtype != torch.float32 and self.head_dim in (64, 128)
                                and hidden % 8 == 0)
         self.device = torch.device(device)
         hd, d, f = self.head_dim, dim, hidden
@@ -66,6 +97,9 @@ class DecoderLayer:
         self.w_ffn_norm = (torch.rand(d, generator=g, device=self.device) + 0.5).to(dtype)
         self.w_gate_up = weight(d, 2 * f)
         self.w_down = weight(f, d)
+        if int8:
+            for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
+                setattr(self, name, Int8Weight(getattr(self, name)))
         self.k_cache = torch.randn(batch, kv_heads, kv_cache_len, hd, generator=g, device=self.device).to(dtype)
         self.v_cache = torch.randn(batch, kv_heads, kv_cache_len, hd, generator=g, device=self.device).to(dtype)
         # activations of one step
@@ -78,11 +112,17 @@ class DecoderLayer:
         self.attn = torch.empty(batch, heads, 1, hd, **e)
         self.o = torch.empty(batch, d, **e)
         self.gate_up = torch.empty(batch if unfused else 0, 2 * f, **e)
-        self.act = torch.empty(batch, f, **e)
+        self.act = Int8Rows(batch, f, self.device) if int8 else torch.empty(batch, f, **e)
         self.down = torch.empty(batch, d, **e)
+        if int8:
+            self.h = Int8Rows(batch, d, self.device)
+            self.h2 = Int8Rows(batch, d, self.device)
+            self.attn_q = Int8Rows(batch, d, self.device)
         ops.rope_table(hd, self.device)  # built before any graph capture
 
     def weights(self) -> dict:
+        """The layer's weights: [in, out] tensors, or with int8 Int8Weight
+        projections ([out, in] rows and scales; ``assign`` quantises others)."""
         return {"w_attn_norm": self.w_attn_norm, "w_qkv": self.w_qkv, "w_o": self.w_o,
                 "w_ffn_norm": self.w_ffn_norm, "w_gate_up": self.w_gate_up, "w_down": self.w_down}
 
@@ -92,6 +132,8 @@ class DecoderLayer:
         updated in place; pending: the previous layer's addend [B, D] or None
         (first layer). Returns this layer's addend (self.down)."""
         b, d, f = self.batch, self.dim, self.hidden
+        if self.int8:
+            return self._decode_int8(x, pending, kv_lens, max_kv_len, is_done)
         if pending is None:
             ops.launch_fused_add_residual_rmsnorm(self.w_attn_norm, x, self.h, False)
             h = self.h
@@ -113,6 +155,34 @@ class DecoderLayer:
         self._gate_up_swiglu(b, self.o, self.gate_up, self.act, fuse)
         ops.launch_linear(False, False, b, d, f, self.act, self.w_down, self.down)
         return self.down
+
+    def _decode_int8(self, x, pending, kv_lens, max_kv_len, is_done):
+        self._norm_int8(self.w_attn_norm, x, pending, self.h)
+        self._product_int8(self.h, self.w_qkv, self.qkv)
+        rope = (ops.launch_fused_reshape_rope_kvcache_llama2_decode if self.pairing
+                else ops.launch_fused_reshape_rope_kvcache_decode)
+        rope(self.qkv, is_done, kv_lens, self.q, self.k_cache, self.v_cache)
+        ops.decode_attention(self.q, self.k_cache, self.v_cache, kv_lens, max_kv_len, self.qk, self.attn)
+        self._after_attention_int8(x, self.attn.view(self.batch, self.dim), self.attn_q, self.o, self.h2, self.gate_up,
+                                   self.act, self.down)
+        return self.down
+
+    @staticmethod
+    def _norm_int8(w, x, addend, rows: Int8Rows):
+        ops.launch_fused_add_residual_rmsnorm_int8(w, x, addend, rows.q, rows.scales, addend is not None)
+
+    @staticmethod
+    def _product_int8(rows: Int8Rows, w: Int8Weight, out):
+        ops.launch_linear_int8(rows.q, rows.scales, w.q, w.scales, out)
+
+    def _after_attention_int8(self, x, attn, attn_q, o, h2, gate_up, act, down):
+        """The O projection and the feed-forward half on int8 rows."""
+        ops.launch_quantize_rows_int8(attn, attn_q.q, attn_q.scales)
+        self._product_int8(attn_q, self.w_o, o)
+        self._norm_int8(self.w_ffn_norm, x, o, h2)
+        self._product_int8(h2, self.w_gate_up, gate_up)
+        ops.launch_swiglu_int8(gate_up, act.q, act.scales)
+        self._product_int8(act, self.w_down, down)
 
     def _fused(self, rows: int) -> bool:
         """Whether this pass uses the epilogue kernels: above 8 rows, where
@@ -153,6 +223,8 @@ class DecoderLayer:
         t, d, f = x.shape[0], self.dim, self.hidden
         qc = unpad_to_pad.numel() // self.batch
         buf = self._prefill_buffers(t, qc)
+        if self.int8:
+            return self._prefill_int8(x, pending, q_lens, kv_lens, max_q, max_kv, unpad_to_pad, buf)
         if pending is None:
             ops.launch_fused_add_residual_rmsnorm(self.w_attn_norm, x, buf["h"], False)
             h = buf["h"]
@@ -177,6 +249,19 @@ class DecoderLayer:
         ops.launch_linear(False, False, t, d, f, buf["act"], self.w_down, buf["down"])
         return buf["down"]
 
+    def _prefill_int8(self, x, pending, q_lens, kv_lens, max_q, max_kv, unpad_to_pad, buf):
+        self._norm_int8(self.w_attn_norm, x, pending, buf["h"])
+        self._product_int8(buf["h"], self.w_qkv, buf["qkv"])
+        rope = (ops.launch_fused_pad_reshape_transpose_rope_kvcache_llama2 if self.pairing
+                else ops.launch_fused_pad_reshape_transpose_rope_kvcache)
+        rope(buf["qkv"], q_lens, kv_lens, unpad_to_pad.view(-1), buf["q"], self.k_cache, self.v_cache)
+        ops.prefill_attention_scores(buf["q"], self.k_cache, q_lens, kv_lens, max_q, max_kv, buf["qk"])
+        ops.launch_attention_qkv(buf["qk"], self.v_cache, buf["pv"], max_q, max_kv)
+        ops.launch_fused_transpose_unpad(x.shape[0], buf["pv"], unpad_to_pad.view(-1), buf["attn"])
+        self._after_attention_int8(x, buf["attn"], buf["attn_q"], buf["o"], buf["h2"], buf["gate_up"], buf["act"],
+                                   buf["down"])
+        return buf["down"]
+
     def _prefill_buffers(self, t: int, qc: int) -> dict:
         key = (t, qc)
         if getattr(self, "_pf_key", None) != key:
@@ -189,11 +274,14 @@ class DecoderLayer:
                         "pv": torch.zeros(b, h, qc, hd, **e), "attn": torch.empty(t, d, **e),
                         "o": torch.empty(t, d, **e), "gate_up": torch.empty(t if unfused else 0, 2 * f, **e),
                         "act": torch.empty(t, f, **e), "down": torch.empty(t, d, **e)}
+            if self.int8:
+                for name, dim in (("h", d), ("h2", d), ("attn_q", d), ("act", f)):
+                    self._pf[name] = Int8Rows(t, dim, self.device)
             self._pf_key = key
         return self._pf
 
     def launches_per_step(self) -> int:
-        return 7 if self._fused(self.batch) else 9
+        return 10 if self.int8 else 7 if self._fused(self.batch) else 9
 
     def launches_per_prefill(self, tokens: int) -> int:
-        return 9 if self._fused(tokens) else 11
+        return 12 if self.int8 else 9 if self._fused(tokens) else 11

@@ -160,6 +160,24 @@ __device__ __forceinline__ float silu_mul(float g, float u)
 }
 
 // ---------------------------------------------------------------------------
+// Programmatic dependent launch: a kernel launched with pdl_attribute() may start
+// while the kernel before it in the stream ends. It touches no global memory before
+// pdl_wait(), which returns once that kernel has completed and its writes are
+// visible; what comes before (barriers, tensor memory, instruction fetch) overlaps
+// the other's end. pdl_trigger() lets the next such kernel start once every CTA of
+// this one has called it or left.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+inline cudaLaunchAttribute pdl_attribute()
+{
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+
+// ---------------------------------------------------------------------------
 // Reductions.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float warp_sum(float v)

@@ -111,6 +111,15 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank)
     return r;
 }
 
+// 16 consecutive accumulator columns of this thread's TMEM lane (no wait).
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+
 // One thread of a converged warp, known to the compiler as one: the tensor-core
 // and TMA instructions behind it are issued once. Behind a comparison with a
 // thread index each took about 80 cycles to issue instead, which set the pace
@@ -287,6 +296,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     };
     int issued = 0; // producers: the group's k blocks whose loads were issued
     constexpr int kAtOnce = 2;
+    pdl_trigger();
     if (warp < groups)
     {
         if (lane < depth)
@@ -296,6 +306,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
+        pdl_wait();
         issued = min(min(count, depth), kAtOnce);
         if (elect_one())
             for (int i = 0; i < issued; ++i)
@@ -317,8 +328,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     else if (warp > 8)
+    {
+        pdl_wait();
         for (int i = tid - 9 * 32; i < bn; i += kTThreads - 9 * 32)
             sb[i] = col0 + i < a.n ? __ldg(a.sb + col0 + i) : 0.f;
+    }
+    pdl_wait(); // (every thread: the epilogue reads scales and writes C)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     }
 
     // warps of the same warp % 4 read TMEM lane quadrant warp % 4: row 32 quad + lane of the
-    // tile, or (BM 64) row 16 quad + lane in lanes 0-15; they share its chunks of 32 columns
+    // tile, or (BM 64) row 16 quad + lane in lanes 0-15; they share its columns, 16 at a time
     const int quad = warp & 3, part = warp >> 2;
     const int lrow = BM == 64 ? 16 * quad + lane : 32 * quad + lane;
     const bool live = (BM == 128 || lane < 16) && row0 + lrow < a.m;
@@ -410,38 +425,43 @@ __global__ void __launch_bounds__(kTThreads, 1)
     }
     __syncwarp();
     tc_fence_after();
-    // the integer sums of accumulator columns [c0, c0 + 32) of this thread's row
-    auto load32 = [&](int c0, uint32_t(&r)[32]) {
+    // the integer sums of accumulator columns [c0, c0 + 16) of this thread's row
+    auto load16 = [&](int c0, uint32_t(&r)[16]) {
         const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)c0;
-        tmem_ld32_async(taddr, r);
-        if (groups == 1)
+        tmem_ld16_async(taddr, r);
+        if (groups > 1)
         {
-            tmem_wait_ld();
-            return;
-        }
-#pragma unroll 1
-        for (int g = 1; g < groups; ++g)
-        {
-            uint32_t x[32];
-            tmem_ld32_async(taddr + (uint32_t)(g * bn), x);
+            uint32_t x[16];
+            tmem_ld16_async(taddr + (uint32_t)bn, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 16; ++e)
                 r[e] += x[e];
         }
+        if (groups > 2)
+        {
+            uint32_t x[16], y[16];
+            tmem_ld16_async(taddr + (uint32_t)(2 * bn), x);
+            tmem_ld16_async(taddr + (uint32_t)(3 * bn), y);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                r[e] += x[e] + y[e];
+        }
+        tmem_wait_ld();
     };
     if (split == 1 && a.wide)
     {
         T *out = static_cast<T *>(a.c) + (row0 + lrow) * a.ldc + col0;
 #pragma unroll 1
-        for (int c0 = 32 * part; c0 < bn; c0 += 128)
+        for (int c0 = 16 * part; c0 < bn; c0 += 64)
         {
-            uint32_t r[32];
-            load32(c0, r);
+            uint32_t r[16];
+            load16(c0, r);
             if (live && !*abort_flag)
             {
 #pragma unroll
-                for (int v = 0; v < 32; v += 8)
+                for (int v = 0; v < 16; v += 8)
                     store8<T>(out + c0 + v, r + v, row_scale, sb + c0 + v, a.n - col0 - c0 - v, true);
             }
             __syncwarp();
@@ -459,15 +479,15 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const int mine = rows_of(rank);
         int *stage = reinterpret_cast<int *>(smem);
 #pragma unroll 1
-        for (int c0 = 32 * part; c0 < bn; c0 += 128)
+        for (int c0 = 16 * part; c0 < bn; c0 += 64)
         {
-            uint32_t r[32];
-            load32(c0, r);
+            uint32_t r[16];
+            load16(c0, r);
             if (live)
             {
                 int4 *dst = reinterpret_cast<int4 *>(stage + lrow * stride + c0);
 #pragma unroll
-                for (int v = 0; v < 8; ++v)
+                for (int v = 0; v < 4; ++v)
                     dst[v] = make_int4((int)r[4 * v], (int)r[4 * v + 1], (int)r[4 * v + 2], (int)r[4 * v + 3]);
             }
             __syncwarp();
@@ -616,8 +636,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
                      "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
+    pdl_trigger();
     tc_fence_before();
     __syncthreads();
+    pdl_wait();
     cluster_barrier(); // both CTAs' barriers are initialized and the tensor memory allocated
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
@@ -923,13 +945,14 @@ int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
     cfg.blockDim = dim3(kTThreads);
     cfg.dynamicSmemBytes = t.smem_bytes;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)split;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1] = pdl_attribute();
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
@@ -967,13 +990,14 @@ int launch_pair(Int8Args a, cudaStream_t stream)
     cfg.blockDim = dim3(kPThreads);
     cfg.dynamicSmemBytes = kPSmemBytes;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1] = pdl_attribute();
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, a);
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8 (two-SM tiles): %s", cudaGetErrorString(e));

@@ -462,6 +462,8 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_kernel(const RowArgs a)
     const T *add = SRC == SRC_NORM_ADD ? static_cast<const T *>(a.residual) + row * a.dim : nullptr;
     T *xio = static_cast<T *>(a.xio) + row * a.dim;
 
+    pdl_trigger();
+    pdl_wait();
     Raw8<T> in[NV], in2[NV], w[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -637,15 +639,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == kTwoPerSM ? 2 : 1)
         }
     };
     int64_t issued = n_mine < depth ? n_mine : depth; // (thread 0's)
+    pdl_trigger();
     if (tid == 0)
     {
         for (int i = 0; i < depth; ++i)
             mbar_init(smem_u32(&s_full[i]), 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        pdl_wait();
         for (int i = 0; i < (int)issued; ++i)
             issue(i, i);
     }
+    pdl_wait();
     // the first element of group j, whose elements are `stride` apart
     const int stride = RAGGED ? n_threads : 1;
     auto at = [&](int j) { return RAGGED ? 8 * j * n_threads + tid : 8 * (j * n_threads + tid); };
@@ -792,6 +797,8 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_any_kernel(const RowArg
         else
             return f;
     };
+    pdl_trigger();
+    pdl_wait();
     Top<V> top;
     float sq = 0.f;
     for (int64_t d = threadIdx.x; d < a.dim; d += blockDim.x)
@@ -819,6 +826,21 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_any_kernel(const RowArg
 }
 
 constexpr int64_t kSmemPerSM = 220 * 1024;
+
+template <typename... P, typename... A>
+int launch_pdl(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = pdl_attribute();
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+    return e == cudaSuccess ? L2K_OK : set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
+}
 
 // CTAs of `threads` threads that an SM's registers hold (allocated in units of
 // 256 for a warp).
@@ -849,8 +871,7 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
     const int64_t grid = std::min<int64_t>(a.n_rows, per_sm * num_sms());
-    kernel<<<(unsigned)grid, threads, (size_t)(depth * stage_bytes), stream>>>(a, depth, (uint32_t)input_bytes);
-    return L2K_OK;
+    return launch_pdl(kernel, (unsigned)grid, threads, (size_t)(depth * stage_bytes), stream, a, depth, (uint32_t)input_bytes);
 }
 
 // Groups per thread: one for the shortest rows (a warp or less); four for 16-bit
@@ -894,15 +915,15 @@ int launch_rows(const RowArgs &a, const char *name, cudaStream_t stream)
     {
         // few rows: latency, so as many threads as there are groups
         if (groups <= kMaxThreads)
-            rows_int8_kernel<T, SRC, 1><<<(unsigned)a.n_rows, (unsigned)(ceil_div(groups, 32) * 32), 0, stream>>>(a);
+            st = launch_pdl(rows_int8_kernel<T, SRC, 1>, (unsigned)a.n_rows, (int)(ceil_div(groups, 32) * 32), 0, stream, a);
         else
-            rows_int8_kernel<T, SRC, 2><<<(unsigned)a.n_rows, (unsigned)(ceil_div(groups, 64) * 32), 0, stream>>>(a);
+            st = launch_pdl(rows_int8_kernel<T, SRC, 2>, (unsigned)a.n_rows, (int)(ceil_div(groups, 64) * 32), 0, stream, a);
     }
     else if (stream_fits)
         st = vec ? launch_stream<T, SRC, false>(a, input_bytes, stage_bytes, stream)
                  : launch_stream<T, SRC, true>(a, input_bytes, stage_bytes, stream);
     else
-        rows_int8_any_kernel<T, SRC><<<(unsigned)a.n_rows, kMaxThreads, 0, stream>>>(a);
+        st = launch_pdl(rows_int8_any_kernel<T, SRC>, (unsigned)a.n_rows, kMaxThreads, 0, stream, a);
     return st != L2K_OK ? st : check_launch(name);
 }
 

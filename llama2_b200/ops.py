@@ -580,10 +580,11 @@ def _int8_rows(q, scales, n, dim, name):
 
 
 def _one_device(*ts) -> int:
-    """The CUDA device that all the tensors are on."""
+    """The CUDA device that all the tensors, contiguous ones, are on."""
     dev = ts[0].get_device()
     for t in ts:
-        if t.get_device() != dev:
+        if t.get_device() != dev or dev < 0 or not t.is_contiguous():
+            _dev(*ts)
             raise ValueError(f"tensors are on different devices: {ts[0].device} and {t.device}")
     return dev
 
@@ -606,10 +607,10 @@ def _raw_stream(dev) -> int:
 def launch_quantize_rows_int8(x, q, scales):
     """Rows to int8: q (N, D) int8 and scales (N,) float32 with
     x[i, j] ~ scales[i] * q[i, j], scales[i] = max_j |x[i, j]| / 127."""
-    _dev(x, q, scales)
+    dev = _one_device(x, q, scales)
     n, dim = x.shape
     _int8_rows(q, scales, n, dim, "q")
-    _call_on(_one_device(x, q, scales), "l2k_quantize_rows_int8", x.data_ptr(), q.data_ptr(), scales.data_ptr(), n,
+    _call_on(dev, "l2k_quantize_rows_int8", x.data_ptr(), q.data_ptr(), scales.data_ptr(), n,
              dim, _code(x))
 
 
@@ -618,7 +619,7 @@ def launch_fused_add_residual_rmsnorm_int8(weights, x, residual, q, scales, add_
     x is updated in place with add_residual; residual is read only (None
     without add_residual)."""
     ts = (weights, x, q, scales, residual) if add_residual else (weights, x, q, scales)
-    _dev(*ts)
+    dev = _one_device(*ts)
     _same(x, weights, "launch_fused_add_residual_rmsnorm_int8")
     n, dim = x.shape
     if add_residual:
@@ -628,19 +629,19 @@ def launch_fused_add_residual_rmsnorm_int8(weights, x, residual, q, scales, add_
     if weights.shape != (dim,):
         raise ValueError("Incorrect rmsnorm weight size")
     _int8_rows(q, scales, n, dim, "q")
-    _call_on(_one_device(*ts), "l2k_fused_add_residual_rmsnorm_int8", weights.data_ptr(), x.data_ptr(),
+    _call_on(dev, "l2k_fused_add_residual_rmsnorm_int8", weights.data_ptr(), x.data_ptr(),
              residual.data_ptr() if add_residual else None, q.data_ptr(), scales.data_ptr(), n, dim,
              int(bool(add_residual)), _code(x))
 
 
 def launch_swiglu_int8(input, q, scales):
     """launch_swiglu with the output rows as int8: input (N, 2F) -> q (N, F), scales (N,)."""
-    _dev(input, q, scales)
+    dev = _one_device(input, q, scales)
     n, f = q.shape
     if input.shape != (n, 2 * f):
         raise ValueError("Incorrect input size")
     _int8_rows(q, scales, n, f, "q")
-    _call_on(_one_device(input, q, scales), "l2k_swiglu_int8", input.data_ptr(), q.data_ptr(), scales.data_ptr(), n, f,
+    _call_on(dev, "l2k_swiglu_int8", input.data_ptr(), q.data_ptr(), scales.data_ptr(), n, f,
              _code(input))
 
 
@@ -648,14 +649,14 @@ def launch_linear_int8(A, a_scales, B, b_scales, C):
     """C = (A B^T) * a_scales[:, None] * b_scales[None, :] for int8 rows: A (M, K)
     with a scale per token, B (N, K) (a weight [out, in]) with a scale per output
     channel, C (M, N) float32, float16 or bfloat16; exact integer sums."""
-    _dev(A, a_scales, B, b_scales, C)
+    dev = _one_device(A, a_scales, B, b_scales, C)
     m, k = A.shape
     n, kb = B.shape
     _int8_rows(A, a_scales, m, k, "A")
     _int8_rows(B, b_scales, n, kb, "B")
     if kb != k or C.shape != (m, n):
         raise ValueError("Matrix sizes do not match")
-    _call_on(_one_device(A, a_scales, B, b_scales, C), "l2k_linear_int8", m, n, k, A.data_ptr(), k,
+    _call_on(dev, "l2k_linear_int8", m, n, k, A.data_ptr(), k,
              a_scales.data_ptr(), B.data_ptr(), k, b_scales.data_ptr(), C.data_ptr(), n, _code(C))
 
 

@@ -62,15 +62,19 @@ def host_tensors(monkeypatch):
     def call(dev, name, *args):
         raise AssertionError(f"{name} was launched")
 
-    monkeypatch.setattr(ops, "_dev", lambda *ts: None)
+    monkeypatch.setattr(ops, "_one_device", lambda *ts: 0)
     monkeypatch.setattr(ops, "_call_on", call)
 
 
 class OnDevice:
     """What _one_device asks of a tensor."""
+    is_cuda = True
 
     def __init__(self, dev):
         self.device = f"cuda:{dev}"
+
+    def is_contiguous(self):
+        return True
 
     def get_device(self):
         return int(self.device[-1])

@@ -635,8 +635,9 @@ int l2k_decode_step_no_alloc(const l2k_decode_step_args *args, l2k_stream_t stre
  *   a (m, k) with row stride lda, b (n, k) with row stride ldb (a weight
  *   [out, in]), c (m, n) of type dtype with row stride ldc. The integer sum is
  *   exact (k <= 131071, else L2K_ERR_UNSUPPORTED_SHAPE; bytes may be any value
- *   from -128 to 127). tcgen05 tensor cores when a and b and their row strides
- *   are multiples of 16 bytes, the CUDA cores otherwise; same results.
+ *   from -128 to 127). tcgen05 tensor cores, fed by TMA when a and b and their
+ *   row strides are multiples of 16 bytes, by plain loads otherwise; same
+ *   results.
  * ------------------------------------------------------------------------ */
 int l2k_quantize_rows_int8(const void *x, int8_t *q, float *scales, int64_t num_rows, int64_t dim, int dtype,
                            l2k_stream_t stream);

@@ -7,14 +7,14 @@
 // Both operands are K-major, so a k block of 128 bytes is one 128-byte
 // swizzled row: the tiles, descriptors and rings are those of a 16-bit
 // product of half the depth (tcgen05.mma.kind::i8, 32 k per instruction).
-// Three kernels:
+// Two kernels:
 //   * linear_int8_tile_kernel: BM x bn tiles (BM 64 or 128, bn 32 .. 256),
 //     K split over a cluster of up to 8 CTAs; for decode batches, bound by
-//     streaming B once, and for short prompts;
+//     streaming B once, and for short prompts; also for operands that TMA cannot
+//     address (a base or a row stride that is no multiple of 16 bytes), whose
+//     rows its idle warps bring to shared memory instead;
 //   * linear_int8_pair_kernel: two SMs per 256 x 256 tile
-//     (cta_group::2), persistent, two accumulators; for prefill;
-//   * linear_int8_any_kernel: CUDA cores (dp4a), any alignment: rows that
-//     TMA cannot address (a base or a row stride that is no multiple of 16).
+//     (cta_group::2), persistent, two accumulators; for prefill.
 // Every mbarrier wait is bounded; on expiry the kernel records an error code
 // (l2k_device_error) and leaves after its copies and MMAs have drained.
 #include "common.cuh"
@@ -50,7 +50,7 @@ __device__ __forceinline__ void int8_fail(int code, volatile int *abort_flag)
 
 struct Int8Args
 {
-    const int8_t *a, *b; // (the CUDA-core kernel)
+    const int8_t *a, *b;
     int64_t lda, ldb;
     const float *sa, *sb;
     void *c;
@@ -252,7 +252,39 @@ __device__ __forceinline__ void bulk_add_s32(uint32_t dst, uint32_t src, uint32_
                  : "memory");
 }
 
-template <typename T, int BM>
+// 16 bytes of a row from any address: those below `valid`, zeros behind. Reads the
+// aligned words around them where these lie in [lo, hi), the operand's bytes.
+__device__ __forceinline__ uint4 load_unaligned16(const int8_t *p, int64_t valid, uintptr_t lo, uintptr_t hi)
+{
+    uint32_t v[4] = {0, 0, 0, 0};
+    const uintptr_t first = (uintptr_t)p & ~(uintptr_t)3;
+    if (valid > 0 && first >= lo && first + 20 <= hi)
+    {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(first);
+        const uint32_t shift = 8 * (uint32_t)((uintptr_t)p & 3);
+        uint32_t x[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            x[i] = __ldg(w + i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            v[i] = __funnelshift_r(x[i], x[i + 1], shift);
+            const int64_t n = valid - 4 * i; // bytes of the word that belong to the row
+            v[i] = n >= 4 ? v[i] : n <= 0 ? 0u : v[i] & ((1u << (8 * n)) - 1);
+        }
+    }
+    else if (valid > 0)
+    {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e < valid)
+                v[e / 4] |= (uint32_t)(uint8_t)p[e] << (8 * (e & 3));
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+template <typename T, int BM, bool TMA>
 __global__ void __launch_bounds__(kTThreads, 1)
     linear_int8_tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                             const __grid_constant__ Int8Args a)
@@ -282,8 +314,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
     const int kb0 = rank * a.kb_per + min(rank, a.kb_more); // the first a.kb_more ranks take one k block more
     const int n_kb = a.kb_per + (rank < a.kb_more ? 1 : 0); // at least `groups`
 
-    // warps 0 .. groups - 1: producers; warps 4 .. 3 + groups: MMA issuers
-    const int group = warp & 3;
+    // warps 0 .. groups - 1: producers (without TMA: all warps but 4 .. 7, 12 / groups to a
+    // group); warps 4 .. 3 + groups: MMA issuers
+    const int group = TMA ? warp & 3 : warp & (groups - 1);
     const int count = group < groups ? (n_kb - group + groups - 1) / groups : 0; // the group's k blocks
     auto issue = [&](int i, int slot) { // the group's i-th k block into its ring's slot
         const int st = slot * groups + group;
@@ -301,17 +334,20 @@ __global__ void __launch_bounds__(kTThreads, 1)
     {
         if (lane < depth)
         {
-            mbar_init(bar_full + 8 * (lane * groups + group), 1);
+            mbar_init(bar_full + 8 * (lane * groups + group), TMA ? 1 : 12 / groups);
             mbar_init(bar_freed + 8 * (lane * groups + group), 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
         pdl_wait();
-        issued = min(min(count, depth), kAtOnce);
-        if (elect_one())
-            for (int i = 0; i < issued; ++i)
-                issue(i, i);
-        __syncwarp();
+        if constexpr (TMA)
+        {
+            issued = min(min(count, depth), kAtOnce);
+            if (elect_one())
+                for (int i = 0; i < issued; ++i)
+                    issue(i, i);
+            __syncwarp();
+        }
     }
     else if (warp == 8)
     {
@@ -339,7 +375,48 @@ __global__ void __launch_bounds__(kTThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp < groups)
+    if (!TMA && (warp < 4 || warp >= 8))
+    {
+        // ---- producers: the tiles' rows by plain loads, 8 lanes to a row's 128 bytes, into
+        // the places that TMA's 128-byte swizzle gives them ----
+        const int helpers = 12 / groups, helper = (warp < 4 ? warp : warp - 4) / groups;
+        const int n_rows = (int)(a.stage_bytes / 128); // bn rows of B, then the rows of A
+        const uintptr_t lo_a = (uintptr_t)a.a, hi_a = lo_a + (a.m - 1) * a.lda + a.k;
+        const uintptr_t lo_b = (uintptr_t)a.b, hi_b = lo_b + (a.n - 1) * a.ldb + a.k;
+        int slot = 0;
+        uint32_t phase = 1; // (a fresh barrier's previous phase counts as complete)
+        for (int i = 0; i < count; ++i)
+        {
+            const int st = slot * groups + group;
+            if (!warp_wait(bar_freed + 8 * st, phase, abort_flag))
+            {
+                int8_fail(ERR_INT8_WAIT_MMA, abort_flag);
+                break;
+            }
+            uint8_t *dst = smem + st * a.stage_bytes;
+            const int64_t kx = (int64_t)(kb0 + i * groups + group) * kBK + 16 * (lane & 7);
+#pragma unroll 4
+            for (int r = 4 * helper + (lane >> 3); r < n_rows; r += 4 * helpers)
+            {
+                const bool of_b = r < bn;
+                const int64_t row = of_b ? col0 + r : row0 + r - bn;
+                const bool in = row < (of_b ? a.n : a.m);
+                const int8_t *p = (of_b ? a.b + row * a.ldb : a.a + row * a.lda) + kx;
+                const uint4 v = load_unaligned16(p, in ? a.k - kx : 0, of_b ? lo_b : lo_a, of_b ? hi_b : hi_a);
+                *reinterpret_cast<uint4 *>(dst + 128 * r + 16 * ((lane & 7) ^ (r & 7))) = v;
+            }
+            fence_proxy_async(); // before the MMAs read them
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(bar_full + 8 * st);
+            if (++slot == depth)
+            {
+                slot = 0;
+                phase ^= 1;
+            }
+        }
+    }
+    else if (TMA && warp < groups)
     {
         // ---- producer: the rest of the group's k blocks ----
         int slot = issued;
@@ -419,7 +496,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     {
         // after a failure the copies and MMAs in flight land before the ring is reused
         const int quiet = 0;
-        for (int i = max(0, issued - depth); i < issued; ++i)
+        for (int i = max(0, issued - depth); i < issued; ++i) // (none without TMA)
             mbar_wait(bar_full + 8 * ((i % depth) * groups + group), (i / depth) & 1, &quiet);
         mbar_wait(bar_done, 0, &quiet);
     }
@@ -781,7 +858,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
                     }
                     fence_proxy_async();
                     __syncwarp();
-                    if (col0 + c0 < a.n && elect_one())
+                    if (col0 + c0 < a.n && row - lane < a.m && elect_one())
                         tma_store_3d(&tm_c, smem_u32(staging), (int)(col0 + c0), (int)(row - lane), 0);
                     bulk_commit(); // (an empty group in the other lanes)
                 }
@@ -836,87 +913,16 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
 }
 
-// ---------------------------------------------------------------------------
-// CUDA cores: 64 x 64 tiles of C, 32 k per step, each thread 4 x 4 sums. Rows
-// may start at any byte; bytes past K are zero.
-// ---------------------------------------------------------------------------
-constexpr int kATileRows = 64, kAStep = 32;
-
+// K = 0: every sum is 0, every element 0 times its scales.
 template <typename T>
-__global__ void __launch_bounds__(256) linear_int8_any_kernel(const Int8Args a)
+__global__ void linear_int8_empty_kernel(const Int8Args a)
 {
-    __shared__ int sa[kAStep / 4][kATileRows + 1], sb[kAStep / 4][kATileRows + 1];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int64_t row0 = (int64_t)blockIdx.y * kATileRows, col0 = (int64_t)blockIdx.x * kATileRows;
-    int acc[4][4] = {};
-    // word w (4 bytes of k) of one of the tile's rows
-    auto word = [&](const int8_t *base, int64_t ld, int64_t row, int64_t rows, int64_t k0) -> int {
-        uint32_t v = 0;
-        if (row < rows)
-            for (int e = 0; e < 4; ++e)
-                if (k0 + e < a.k)
-                    v |= (uint32_t)(uint8_t)base[row * ld + k0 + e] << (8 * e);
-        return (int)v;
-    };
-    for (int64_t k0 = 0; k0 < a.k; k0 += kAStep)
-    {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-        {
-            const int w = tid & 7, r = (tid >> 3) + 32 * i;
-            sa[w][r] = word(a.a, a.lda, row0 + r, a.m, k0 + 4 * w);
-            sb[w][r] = word(a.b, a.ldb, col0 + r, a.n, k0 + 4 * w);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kAStep / 4; ++w)
-        {
-            int x[4], y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                x[i] = sa[w][ty + 16 * i];
-                y[i] = sb[w][tx + 16 * i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __dp4a(x[i], y[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-        {
-            const int64_t row = row0 + ty + 16 * i, col = col0 + tx + 16 * j;
-            if (row < a.m && col < a.n)
-                static_cast<T *>(a.c)[row * a.ldc + col] =
-                    from_f<T>(__fmul_rn((float)acc[i][j], __fmul_rn(a.sa[row], a.sb[col])));
-        }
+    for (int64_t row = blockIdx.y; row < a.m; row += gridDim.y)
+        for (int64_t col = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; col < a.n; col += (int64_t)gridDim.x * blockDim.x)
+            static_cast<T *>(a.c)[row * a.ldc + col] = from_f<T>(__fmul_rn(0.f, __fmul_rn(a.sa[row], a.sb[col])));
 }
 
-template <typename T>
-int launch_any(const Int8Args &a, cudaStream_t stream)
-{
-    // gridDim.y is limited to 65535: longer products go in slabs of rows
-    const int64_t slab = (int64_t)65535 * kATileRows;
-    for (int64_t r = 0; r < a.m; r += slab)
-    {
-        Int8Args s = a;
-        s.m = std::min(slab, a.m - r);
-        s.a = a.a + r * a.lda;
-        s.sa = a.sa + r;
-        s.c = static_cast<T *>(a.c) + r * a.ldc;
-        const dim3 grid((unsigned)ceil_div(a.n, kATileRows), (unsigned)ceil_div(s.m, kATileRows));
-        linear_int8_any_kernel<T><<<grid, 256, 0, stream>>>(s);
-    }
-    return check_launch("l2k_linear_int8");
-}
-
-template <typename T, int BM>
+template <typename T, int BM, bool TMA>
 int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
 {
     while (groups > 1 && (groups * bn > 512 || groups > a.n_kb / split)) // 512 TMEM columns, a k block for each
@@ -930,13 +936,13 @@ int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
     a.stages = t.stages;
     a.stage_bytes = t.stage_bytes;
     a.ring_bytes = t.ring_bytes;
-    CUtensorMap ma, mb;
+    CUtensorMap ma = {}, mb = {};
     const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const uint64_t m = (uint64_t)a.m, n = (uint64_t)a.n, k = (uint64_t)a.k, lda = (uint64_t)a.lda, ldb = (uint64_t)a.ldb;
-    if (!make_map(&ma, dt, a.a, k, m, 1, lda, lda * m, (uint32_t)t.a_rows, kBK) ||
-        !make_map(&mb, dt, a.b, k, n, 1, ldb, ldb * n, (uint32_t)bn, kBK))
+    if (TMA && (!make_map(&ma, dt, a.a, k, m, 1, lda, lda * m, (uint32_t)t.a_rows, kBK) ||
+                !make_map(&mb, dt, a.b, k, n, 1, ldb, ldb * n, (uint32_t)bn, kBK)))
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
-    auto kernel = linear_int8_tile_kernel<T, BM>;
+    auto kernel = linear_int8_tile_kernel<T, BM, TMA>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTMaxSmem);
     if (e != cudaSuccess)
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
@@ -1024,7 +1030,7 @@ int resident_clusters(int split)
     int &c = cache[dev][split];
     if (c == 0)
     {
-        auto kernel = linear_int8_tile_kernel<T, 128>;
+        auto kernel = linear_int8_tile_kernel<T, 128, true>;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)split);
         cfg.blockDim = dim3(kTThreads);
@@ -1055,8 +1061,9 @@ int resident_clusters(int split)
 // from HBM, and 0.62 of the shorter of the two on top of the longer; then 5300 for
 // launch, first loads and teardown, and for the reduction over a cluster 740 and a
 // quarter of the tile's elements. The two-SM kernel: 438 a k block, 11000 once.
+// Without TMA only the tile kernel, at 15 bytes per clock for what its warps move.
 template <typename T>
-Plan estimate(int64_t m, int64_t n, int n_kb)
+Plan estimate(int64_t m, int64_t n, int n_kb, bool tma)
 {
     const int64_t pairs = num_sms() / 2;
     const double dram = ((double)(m + n) * n_kb * kBK + 2.0 * m * n) / 3657.0;
@@ -1065,8 +1072,14 @@ Plan estimate(int64_t m, int64_t n, int n_kb)
     double best_t = together((double)ceil_div(ceil_div(m, 256) * ceil_div(n, 256), pairs) * n_kb * 438.0) + 11040.0;
     const int bm = m <= 64 ? 64 : 128;
     const int64_t mt = ceil_div(m, bm), a_rows = std::min<int64_t>(bm, ceil_div(m, 8) * 8);
-    if (mt > 65535 || ceil_div(n, 32) > 65535 || mt * ceil_div(n, 256) > 16 * pairs)
+    if (tma && (mt > 65535 || ceil_div(n, 32) > 65535 || mt * ceil_div(n, 256) > 16 * pairs))
         return best; // (many tiles: far in the two-SM kernel's range)
+    if (!tma)
+    {
+        best = Plan{bm, 256, 1, 2};
+        best_t = 1e300;
+    }
+    const double move = tma ? 79.0 : 15.0;
     for (int bn = 32; bn <= 256; bn += 32)
         for (int split = 1; split <= 8 && split <= n_kb; ++split)
         {
@@ -1078,7 +1091,7 @@ Plan estimate(int64_t m, int64_t n, int n_kb)
             {
                 if (groups > 1 && groups > n_kb / split)
                     continue;
-                const double kb = std::max({2.0 * bn, 450.0 / groups, (double)(bn + a_rows) * 128 / 79.0});
+                const double kb = std::max({2.0 * bn, 450.0 / groups, (double)(bn + a_rows) * 128 / move});
                 const double run = waves * (per * kb + (15.5 + 2.2 * (groups - 1)) * bn);
                 const double t = together(run) + 5337.0 + (split > 1 ? 737.0 + 0.255 * bm * bn : 0.0);
                 if (t < best_t)
@@ -1089,7 +1102,7 @@ Plan estimate(int64_t m, int64_t n, int n_kb)
             }
             if (bn < 128 && n_kb / split < 2) // too few k blocks for two groups
             {
-                const double run = waves * (per * 450.0 + 15.5 * bn);
+                const double run = waves * (per * std::max(450.0, (double)(bn + a_rows) * 128 / move) + 15.5 * bn);
                 const double t = together(run) + 5337.0 + (split > 1 ? 737.0 + 0.255 * bm * bn : 0.0);
                 if (t < best_t)
                 {
@@ -1104,24 +1117,31 @@ Plan estimate(int64_t m, int64_t n, int n_kb)
 // estimate(), remembered for the sizes last asked for (a pure function of them and
 // the device's SM count).
 template <typename T>
-Plan plan(int64_t m, int64_t n, int n_kb)
+Plan plan(int64_t m, int64_t n, int n_kb, bool tma)
 {
     struct Entry
     {
         int64_t m = -1, n = 0;
         int n_kb = 0;
+        bool tma = false;
         Plan p{};
     };
     static thread_local Entry cache[64];
     Entry &e = cache[(uint64_t)(m * 31 + n * 7 + n_kb) % 64];
-    if (e.m != m || e.n != n || e.n_kb != n_kb)
-    {
-        e.p = estimate<T>(m, n, n_kb);
-        e.m = m;
-        e.n = n;
-        e.n_kb = n_kb;
-    }
+    if (e.m != m || e.n != n || e.n_kb != n_kb || e.tma != tma)
+        e = Entry{m, n, n_kb, tma, estimate<T>(m, n, n_kb, tma)};
     return e.p;
+}
+
+template <typename T, bool TMA>
+int launch_planned(const Int8Args &a, cudaStream_t stream)
+{
+    const Plan t = plan<T>(a.m, a.n, a.n_kb, TMA);
+    if (t.bm == 64)
+        return launch_tile<T, 64, TMA>(a, t.bn, t.split, t.groups, stream);
+    if (t.bm == 128)
+        return launch_tile<T, 128, TMA>(a, t.bn, t.split, t.groups, stream);
+    return launch_pair<T>(a, stream); // (only with TMA)
 }
 
 template <typename T>
@@ -1130,16 +1150,36 @@ int launch_linear(const Int8Args &p, cudaStream_t stream)
     Int8Args a = p;
     a.wide = (a.ldc * (int64_t)sizeof(T)) % 16 == 0 && is_aligned(a.c, 16);
     a.n_kb = (int)ceil_div(a.k, kBK);
-    const bool tc = a.k > 0 && is_aligned(a.a, 16) && is_aligned(a.b, 16) && a.lda % 16 == 0 && a.ldb % 16 == 0 &&
-                    encode_fn() != nullptr;
-    if (!tc)
-        return launch_any<T>(a, stream);
-    const Plan t = plan<T>(a.m, a.n, a.n_kb);
-    if (t.bm == 64)
-        return launch_tile<T, 64>(a, t.bn, t.split, t.groups, stream);
-    if (t.bm == 128)
-        return launch_tile<T, 128>(a, t.bn, t.split, t.groups, stream);
-    return launch_pair<T>(a, stream);
+    if (a.k == 0)
+    {
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(a.n, 256), 1024), (unsigned)std::min<int64_t>(a.m, 65535));
+        linear_int8_empty_kernel<T><<<grid, 256, 0, stream>>>(a);
+        return check_launch("l2k_linear_int8");
+    }
+    if (is_aligned(a.a, 16) && is_aligned(a.b, 16) && a.lda % 16 == 0 && a.ldb % 16 == 0)
+    {
+        if (encode_fn() == nullptr)
+            return set_error(L2K_ERR_CUDA, "l2k_linear_int8: the driver has no tensor map encoder");
+        return launch_planned<T, true>(a, stream);
+    }
+    // operands that TMA cannot address: slabs of rows and columns within the grid's limits
+    const int64_t rows = (int64_t)65535 * 64, cols = (int64_t)65535 * 32;
+    for (int64_t r = 0; r < a.m; r += rows)
+        for (int64_t c = 0; c < a.n; c += cols)
+        {
+            Int8Args s = a;
+            s.m = std::min(rows, a.m - r);
+            s.n = std::min(cols, a.n - c);
+            s.a = a.a + r * a.lda;
+            s.b = a.b + c * a.ldb;
+            s.sa = a.sa + r;
+            s.sb = a.sb + c;
+            s.c = static_cast<T *>(a.c) + r * a.ldc + c;
+            const int st = launch_planned<T, false>(s, stream);
+            if (st != L2K_OK)
+                return st;
+        }
+    return L2K_OK;
 }
 
 } // namespace

@@ -280,13 +280,31 @@ def test_linear_on_tensor_cores(m, n, k):
         assert (store[m * n:] == 3.0).all()
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 70, 17), (65, 129, 1001), (2, 5, 4093), (130, 64, 63)])
-def test_linear_on_cuda_cores(m, n, k):
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 70, 17), (65, 129, 1001), (2, 5, 4093), (130, 64, 63), (1, 4096, 4095),
+                                   (64, 300, 2050), (300, 1000, 515), (1000, 257, 1300)])
+def test_linear_without_tma(m, n, k):
     """Rows of no multiple of 16 bytes."""
     a, sa, b, sb = operands(m, n, k, k)
     for dtype in DTYPES:
         c = torch.empty(m, n, dtype=dtype, device="cuda")
         ops.launch_linear_int8(a, sa, b, sb, c)
+        check_product(c, a, sa, b, sb)
+
+
+@pytest.mark.parametrize("m,k", [(3, 4099), (70, 77)])
+def test_linear_without_tma_reads_its_rows_alone(m, k):
+    """Rows between bytes of other values, at every offset from a word."""
+    n = 37
+    a, sa, b, sb = operands(m, n, k, 9)
+    for lda, ldb, at in ((k + 1, k + 2, 1), (k + 3, k, 2), (k, k + 5, 3)):
+        bufs = []
+        for t, rows, ld in ((a, m, lda), (b, n, ldb)):
+            buf = torch.full((rows * ld + 8,), -77, dtype=torch.int8, device="cuda")
+            buf[at:at + rows * ld].view(rows, ld)[:, :k] = t
+            bufs.append(buf)
+        c = torch.empty(m, n, device="cuda")
+        capi.call("l2k_linear_int8", m, n, k, bufs[0].data_ptr() + at, lda, sa.data_ptr(), bufs[1].data_ptr() + at, ldb,
+                  sb.data_ptr(), c.data_ptr(), n, capi.L2K_F32, torch.cuda.current_stream().cuda_stream)
         check_product(c, a, sa, b, sb)
 
 

@@ -170,9 +170,9 @@ __device__ __forceinline__ Quantizer<V> make_quantizer(Bits top, float inv_rms)
 // quotient of a 32- and a 24-bit integer that is no border between two integers
 // is further from one than fp64 rounds.
 template <typename V>
-__device__ __noinline__ uint32_t quantize_divided(V y, V a, bool dead)
+__device__ __noinline__ uint32_t quantize_divided(V y, V a)
 {
-    return dead ? 0u : (uint32_t)__double2int_rn(__ddiv_rn(__dmul_rn((double)y, 127.0), (double)a));
+    return (uint32_t)__double2int_rn(__ddiv_rn(__dmul_rn((double)y, 127.0), (double)a));
 }
 
 // The same for a value that lies next to the border k + 1/2, k >= 0: which side.
@@ -185,7 +185,7 @@ __device__ __noinline__ uint32_t quantize_at_border(float y, float a, float r)
 }
 __device__ __forceinline__ uint32_t quantize_at_border(double y, double a, float)
 {
-    return quantize_divided(y, a, false);
+    return quantize_divided(y, a);
 }
 
 // Two fp32 operations at once.
@@ -237,8 +237,10 @@ constexpr bool kShort = SRC != SRC_SWIGLU &&
 template <bool SHORT, typename V>
 __device__ __forceinline__ uint32_t quantize1(V y, const Quantizer<V> &z)
 {
+    if (z.dead)
+        return 0u;
     if (z.r == 0.f)
-        return quantize_divided(y, z.a, z.dead);
+        return quantize_divided(y, z.a);
     if constexpr (SHORT)
         return __float_as_uint(__fadd_rn(__fmaf_rn(y, z.r, __fmul_rn(y, z.r_lo)), kMagic));
     else
@@ -254,12 +256,14 @@ __device__ __forceinline__ uint32_t quantize1(V y, const Quantizer<V> &z)
 template <bool SHORT, typename V>
 __device__ __forceinline__ uint2 quantize8(const V (&y)[8], const Quantizer<V> &z)
 {
+    if (z.dead) // (the whole row; padding is common)
+        return make_uint2(0u, 0u);
     uint32_t b[8];
     if (z.r == 0.f) // (the whole row)
     {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            b[e] = quantize_divided(y[e], z.a, z.dead);
+            b[e] = quantize_divided(y[e], z.a);
     }
     else
     {

@@ -127,7 +127,7 @@ def test_launch_on_the_tensors_device(monkeypatch):
         def __exit__(self, *a):
             current[0] = self.old
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(ops, "_current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(ops, "_raw_stream", lambda dev: 100 + dev)
     monkeypatch.setattr(capi, "call", lambda name, *args: calls.append((current[0], name, *args)))

@@ -533,7 +533,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 // so that a warp's element accesses are to neighbours.
 constexpr int kMaxDepth = 8;
 constexpr int kStreamThreads = 512;
-constexpr int kTwoPerSM = 448; // threads of the instantiation held to 72 registers, so that an SM takes two CTAs
 
 __device__ __forceinline__ uintptr_t down16(uintptr_t p) { return p & ~(uintptr_t)15; }
 __device__ __forceinline__ uintptr_t up16(uintptr_t p) { return (p + 15) & ~(uintptr_t)15; }
@@ -604,8 +603,10 @@ __device__ __forceinline__ void scatter8(B *p, const B (&v)[8], int e, int strid
     }
 }
 
+// THREADS: the most threads of a launch; below kStreamThreads the instantiation is held
+// to the registers with which an SM takes two such CTAs (448: 72, 320: 96).
 template <typename T, int SRC, int NV, bool RAGGED, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == kTwoPerSM ? 2 : 1)
+__global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
     rows_int8_stream_kernel(const RowArgs a, const int depth, const uint32_t input_bytes)
 {
     using V = typename RowValue<T, SRC>::type;
@@ -846,8 +847,8 @@ int launch_pdl(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cu
     return e == cudaSuccess ? L2K_OK : set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
 }
 
-// CTAs of `threads` threads that an SM's registers hold (allocated in units of
-// 256 for a warp).
+// CTAs of `threads` threads that an SM's registers hold: 16384 in each of its four
+// parts, allocated in units of 256 for a warp.
 template <typename T, int SRC, int NV, bool RAGGED, int THREADS>
 int stream_resident(int threads)
 {
@@ -856,7 +857,7 @@ int stream_resident(int threads)
         return cudaFuncGetAttributes(&f, rows_int8_stream_kernel<T, SRC, NV, RAGGED, THREADS>) == cudaSuccess ? f.numRegs
                                                                                                               : 128;
     }();
-    return std::max(1, 65536 / ((regs * 32 + 255) / 256 * 256 * (threads / 32)));
+    return std::max(1, 4 * (16384 / ((regs * 32 + 255) / 256 * 256)) / (threads / 32));
 }
 
 // The stream kernel on as many CTAs as an SM holds, with a ring that keeps about
@@ -883,8 +884,11 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
 // four groups: 16384 x 4096 bf16 rows 40 us, 44 with two), two where a few rows per
 // SM leave threads idle (512 rows: 4.0 us, 4.7 with one); two for fp32 rows (53 us,
 // 60 with four) and one for fp32 SwiGLU (90 us, 99 with two) and a few ragged
-// rows; more where the row needs it. SwiGLU rows of 416 to 448 threads would leave
-// an SM one CTA at their 77 registers: 4099 x 13824 f16 75 us, 61 with two.
+// rows; more where the row needs it. CTAs of 352 to 448 threads would leave an SM
+// one of them at the 86 to 96 registers of the plain instantiation: 4099 x 13824 f16
+// SwiGLU 75 us, 56 with two; 8192 x 11008 bf16 rows 74, 55 with two; likewise fp32
+// norms of 288 to 320 threads (8192 x 5120: 114 us, 100 with two). 16-bit norms stay at
+// their 122 to 126: held to 80 they spill (16384 x 4096: 94 us against 76).
 template <typename T, int SRC, bool RAGGED>
 int launch_stream(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes, cudaStream_t stream)
 {
@@ -896,11 +900,14 @@ int launch_stream(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes, cu
                                                                                      : 4;
     if (want == 1 && groups <= kStreamThreads)
         return launch_stream_nv<T, SRC, 1, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
+    if constexpr (kNorm && kWide && !RAGGED)
+        if (groups > 2 * 256 && groups <= 2 * 320)
+            return launch_stream_nv<T, SRC, 2, RAGGED, 320>(a, input_bytes, stage_bytes, stream);
     if (want <= 2 && groups <= 2 * kStreamThreads)
         return launch_stream_nv<T, SRC, 2, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
-    if constexpr (!kWide && SRC == SRC_SWIGLU && !RAGGED)
-        if (groups > 4 * 384 && groups <= 4 * kTwoPerSM)
-            return launch_stream_nv<T, SRC, 4, RAGGED, kTwoPerSM>(a, input_bytes, stage_bytes, stream);
+    if constexpr (!kNorm && !RAGGED)
+        if (groups > 4 * 320 && groups <= 4 * 448)
+            return launch_stream_nv<T, SRC, 4, RAGGED, 448>(a, input_bytes, stage_bytes, stream);
     return launch_stream_nv<T, SRC, 4, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
 }
 

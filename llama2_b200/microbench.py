@@ -7,7 +7,8 @@ current stream; ``gemm`` times back-to-back launches of the products of
 more than 128 rows (compute-bound, L2 irrelevant) and flushed launches of
 the decode-sized ones (at most 128 rows: bound by reading B, whose 34-180 MB
 would otherwise sit in L2 between launches), next to ``torch.matmul`` on the
-same operands (cuBLAS, for reference); the others flush L2 before every
+same operands (cuBLAS, for reference); ``int8`` times its products likewise
+(flushed up to 1024 rows); the others flush L2 before every
 timed launch (write a 512 MB buffer, then read another, outside the timed
 window). Inputs are seeded
 random tensors of the 7B shapes.

@@ -9,7 +9,9 @@ is launched. Work is enqueued on torch's current CUDA stream through the C
 ABI (llama2_b200.capi); nothing here computes on the CPU.
 
 Integer tensors (ids, lengths, index maps) are 4-byte (torch.uint32 or
-torch.int32, read as unsigned); masks and done flags are torch.uint8.
+torch.int32, read as unsigned); masks and done flags are torch.uint8; the
+8-bit operators (launch_*_int8) take torch.int8 rows with float32 scales and
+run on the device of their tensors.
 """
 from __future__ import annotations
 

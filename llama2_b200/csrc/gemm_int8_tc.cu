@@ -913,6 +913,14 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
 }
 
+int cuda_status(cudaError_t e)
+{
+    if (e == cudaSuccess)
+        return L2K_OK;
+    (void)cudaGetLastError(); // (else the next launch would report it again)
+    return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
+}
+
 // K = 0: every sum is 0, every element 0 times its scales.
 template <typename T>
 __global__ void linear_int8_empty_kernel(const Int8Args a)
@@ -943,9 +951,9 @@ int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
                 !make_map(&mb, dt, a.b, k, n, 1, ldb, ldb * n, (uint32_t)bn, kBK)))
         return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
     auto kernel = linear_int8_tile_kernel<T, BM, TMA>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTMaxSmem);
-    if (e != cudaSuccess)
-        return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
+    const int st = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTMaxSmem));
+    if (st != L2K_OK)
+        return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)split, (unsigned)ceil_div(a.n, bn), (unsigned)ceil_div(a.m, BM));
     cfg.blockDim = dim3(kTThreads);
@@ -959,10 +967,7 @@ int launch_tile(Int8Args a, int bn, int split, int groups, cudaStream_t stream)
     attr[1] = pdl_attribute();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, a);
-    if (e != cudaSuccess)
-        return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
-    return check_launch("l2k_linear_int8");
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ma, mb, a));
 }
 
 // The two-SM kernel: 256 x 256 tiles over clusters of two CTAs.
@@ -987,9 +992,10 @@ int launch_pair(Int8Args a, cudaStream_t stream)
             return set_error(L2K_ERR_CUDA, "l2k_linear_int8: tensor map encoding failed");
     }
     auto kernel = linear_int8_pair_kernel<T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmemBytes);
-    if (e != cudaSuccess)
-        return set_error(L2K_ERR_CUDA, "l2k_linear_int8: %s", cudaGetErrorString(e));
+    const int st =
+        cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPSmemBytes));
+    if (st != L2K_OK)
+        return st;
     const int64_t tiles = ceil_div(a.m, 256) * a.n_nt;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, num_sms() / 2)));
@@ -1004,10 +1010,7 @@ int launch_pair(Int8Args a, cudaStream_t stream)
     attr[1] = pdl_attribute();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, a);
-    if (e != cudaSuccess)
-        return set_error(L2K_ERR_CUDA, "l2k_linear_int8 (two-SM tiles): %s", cudaGetErrorString(e));
-    return check_launch("l2k_linear_int8 (two-SM tiles)");
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, a));
 }
 
 // Which kernel, and its tiles.
@@ -1211,6 +1214,8 @@ extern "C" int l2k_linear_int8(int64_t m, int64_t n, int64_t k, const int8_t *a,
     if (m == 0 || n == 0)
         return L2K_OK;
     L2K_REQUIRE(a_scales && b_scales && c && (k == 0 || (a && b)), "l2k_linear_int8: null pointer");
+    L2K_REQUIRE(is_aligned(a_scales, 4) && is_aligned(b_scales, 4) && is_aligned(c, dtype_size(dtype)),
+                "l2k_linear_int8: c or the scales are not aligned to their elements");
     L2K_REQUIRE_SHAPE(k <= kMaxK, "l2k_linear_int8: k > %d could overflow a 32-bit sum", kMaxK);
     L2K_REQUIRE_SHAPE(m < (int64_t(1) << 31) && n < (int64_t(1) << 31) &&
                           ceil_div(m, 64) * ceil_div(n, 32) < (int64_t(1) << 28),

@@ -832,6 +832,14 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_any_kernel(const RowArg
 
 constexpr int64_t kSmemPerSM = 220 * 1024;
 
+int cuda_status(cudaError_t e)
+{
+    if (e == cudaSuccess)
+        return L2K_OK;
+    (void)cudaGetLastError(); // (else the next launch would report it again)
+    return set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
+}
+
 template <typename... P, typename... A>
 int launch_pdl(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t stream, A... args)
 {
@@ -843,8 +851,7 @@ int launch_pdl(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cu
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
-    return e == cudaSuccess ? L2K_OK : set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
 }
 
 // CTAs of `threads` threads that an SM's registers hold: 16384 in each of its four
@@ -872,9 +879,10 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
     const int64_t per_sm = std::max<int64_t>(1, std::min(resident, kSmemPerSM / (2 * stage_bytes)));
     const int64_t fits = kSmemPerSM / (per_sm * stage_bytes); // at least 1 (stage_bytes <= kSmemPerSM)
     const int depth = (int)std::min({std::max<int64_t>(96 * 1024 / (per_sm * stage_bytes), 2), fits, (int64_t)kMaxDepth});
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemPerSM);
-    if (e != cudaSuccess)
-        return set_error(L2K_ERR_CUDA, "int8 rows: %s", cudaGetErrorString(e));
+    const int st = cuda_status(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemPerSM));
+    if (st != L2K_OK)
+        return st;
     const int64_t grid = std::min<int64_t>(a.n_rows, per_sm * num_sms());
     return launch_pdl(kernel, (unsigned)grid, threads, (size_t)(depth * stage_bytes), stream, a, depth, (uint32_t)input_bytes);
 }
@@ -950,9 +958,12 @@ int check_rows(const RowArgs &a, int dtype, const char *name, cudaStream_t strea
     L2K_REQUIRE(a.scales, "%s: null pointer", name);
     if (a.dim == 0) // rows without elements: scale 0
     {
-        const cudaError_t e = cudaMemsetAsync(a.scales, 0, (size_t)a.n_rows * sizeof(float), stream);
-        return e == cudaSuccess ? L2K_OK : set_error(L2K_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+        return cuda_status(cudaMemsetAsync(a.scales, 0, (size_t)a.n_rows * sizeof(float), stream));
     }
+    const uintptr_t es = dtype_size(dtype);
+    L2K_REQUIRE(is_aligned(a.x, es) && is_aligned(a.xio, es) && is_aligned(a.residual, es) && is_aligned(a.w, es) &&
+                    is_aligned(a.scales, 4),
+                "%s: a tensor is not aligned to its elements", name);
     L2K_REQUIRE_SHAPE(a.n_rows < (int64_t(1) << 31), "%s: more than 2^31 - 1 rows", name);
     *done = false;
     return L2K_OK;

@@ -626,6 +626,7 @@ def launch_fused_add_residual_rmsnorm_int8(weights, x, residual, q, scales, add_
     """launch_fused_add_residual_rmsnorm with the normed rows as int8 (q, scales):
     x is updated in place with add_residual; residual is read only (None
     without add_residual)."""
+    _require(residual is not None or not add_residual, "add_residual needs a residual")
     ts = (weights, x, q, scales, residual) if add_residual else (weights, x, q, scales)
     dev = _one_device(*ts)
     _same(x, weights, "launch_fused_add_residual_rmsnorm_int8")

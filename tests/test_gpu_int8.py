@@ -266,7 +266,11 @@ def check_product(c, a, sa, b, sb):
 LINEAR = [(1, 1, 16), (1, 64, 128), (1, 4096, 4096), (2, 33, 48), (7, 100, 400), (8, 96, 272), (9, 1000, 1040),
           (63, 4100, 512), (64, 12288, 1024), (64, 320, 11008), (65, 257, 144), (100, 4096, 2048), (127, 513, 640),
           (128, 22016, 256), (129, 1003, 2064), (200, 4096, 1040), (255, 700, 4096), (256, 256, 128),
-          (257, 1003, 2064), (300, 31, 4096), (511, 2049, 16), (1000, 1537, 1296), (2048, 4096, 4096)]
+          (257, 1003, 2064), (300, 31, 4096), (511, 2049, 16), (1000, 1537, 1296), (2048, 4096, 4096),
+          (2100, 4099, 528), (3333, 5000, 400), (5000, 2056, 1024)]
+
+
+LINEAR_MIX = [(1, 4096, 1024), (64, 4096, 2048), (70, 300, 1001), (2048, 4096, 512), (130, 1000, 640)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEAR)
@@ -344,6 +348,23 @@ def test_linear_of_the_largest_sums(m, k):
     ops.launch_linear_int8(a, one, b, one[:1].expand(3).contiguous(), c)
     want = torch.tensor([16384 * k, -16256 * k, 16384 * k], dtype=torch.float64, device="cuda").float()
     assert torch.equal(c, want.expand(m, 3))
+
+
+def test_products_on_two_streams():
+    """Launches of all kinds on two streams at once, each ten times in a row."""
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    work = [[operands(*shape, seed) for shape in LINEAR_MIX] for seed in (1, 2)]
+    outs = [[torch.empty(o[0].shape[0], o[2].shape[0], dtype=torch.bfloat16, device="cuda") for o in w] for w in work]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, w, cs in zip(streams, work, outs):
+            with torch.cuda.stream(s):
+                for (a, sa, b, sb), c in zip(w, cs):
+                    ops.launch_linear_int8(a, sa, b, sb, c)
+    torch.cuda.synchronize()
+    for w, cs in zip(work, outs):
+        for o, c in zip(w, cs):
+            check_product(c, *o)
 
 
 @pytest.mark.parametrize("m", [4, 300])

@@ -39,6 +39,13 @@ BF16, F32 = capi.L2K_BF16, capi.L2K_F32
     ("l2k_linear_int8", (4, 8, 32, 16, 32, 16, 16, 32, None, 16, 8, BF16, None), 1),
     ("l2k_linear_int8", (4, 8, 32, 16, 32, 16, 16, 32, 16, None, 8, BF16, None), 1),
     ("l2k_linear_int8", (4, 8, 131072, 16, 131072, 16, 16, 131072, 16, 16, 8, BF16, None), 3),  # sums past 2^31
+    ("l2k_quantize_rows_int8", (18, 16, 16, 4, 8, F32, None), 1),  # not aligned to its elements
+    ("l2k_quantize_rows_int8", (16, 16, 18, 4, 8, BF16, None), 1),
+    ("l2k_fused_add_residual_rmsnorm_int8", (17, 32, 48, 16, 16, 2, 8, 1, BF16, None), 1),
+    ("l2k_fused_add_residual_rmsnorm_int8", (16, 32, 49, 16, 16, 2, 8, 1, BF16, None), 1),
+    ("l2k_swiglu_int8", (17, 16, 16, 2, 4, BF16, None), 1),
+    ("l2k_linear_int8", (4, 8, 32, 16, 32, 16, 16, 32, 16, 17, 8, BF16, None), 1),
+    ("l2k_linear_int8", (4, 8, 32, 16, 32, 18, 16, 32, 16, 16, 8, BF16, None), 1),
     ("l2k_linear_int8", (2 ** 31, 8, 32, 16, 32, 16, 16, 32, 16, 16, 8, BF16, None), 3),
 ])
 def test_c_abi_refuses(call, args, status):
@@ -98,6 +105,7 @@ def f32(*s):
     lambda: ops.launch_fused_add_residual_rmsnorm_int8(f32(7), f32(3, 8), None, i8(3, 8), f32(3), False),
     lambda: ops.launch_fused_add_residual_rmsnorm_int8(f32(8).half(), f32(3, 8), None, i8(3, 8), f32(3), False),
     lambda: ops.launch_fused_add_residual_rmsnorm_int8(f32(8), f32(3, 8), f32(3, 8).half(), i8(3, 8), f32(3), True),
+    lambda: ops.launch_fused_add_residual_rmsnorm_int8(f32(8), f32(3, 8), None, i8(3, 8), f32(3), True),
     lambda: ops.launch_swiglu_int8(f32(3, 8), i8(3, 8), f32(3)),
     lambda: ops.launch_swiglu_int8(f32(3, 16), i8(3, 8), f32(2)),
     lambda: ops.launch_linear_int8(i8(3, 32), f32(3), i8(5, 16), f32(5), f32(3, 5)),

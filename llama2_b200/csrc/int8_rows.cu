@@ -525,82 +525,69 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 // halves). A stage is refilled once the row's reduction has shown that every
 // thread has read it. Each thread holds NV groups of 8 elements.
 //
-// Aligned rows (16-byte aligned, a multiple of 8 elements): groups of 8
-// neighbours, 16-byte accesses. RAGGED: rows of any length and alignment. The copy
-// takes the 16-byte units that the row touches (bytes of the rows next to it are
-// not used), except units that reach out of the tensor, whose elements are read
-// from global memory; element i of group j of thread t is (8 j + i) threads + t,
-// so that a warp's element accesses are to neighbours.
+// Aligned rows (16-byte aligned, a multiple of 8 elements): 16-byte accesses.
+// RAGGED: rows of any length and alignment, in 16-byte accesses too (an element at a
+// time, 16384 x 1023 bf16 rows took 25 us, norms 61, SwiGLU 41; now 20, 39, 32; 4099 x
+// 13799: 82, 197, 126, now 46, 114, 85):
+// - A CTA's rows lie a multiple of 8 rows apart, so all of them lie alike with respect
+//   to the units of 8 elements in memory.
+// - The groups are cut where q's bytes (norms: the row that is written back) can be
+//   stored together. The first group may begin before the row and the last end behind
+//   it; where the two parts fit into one group they share the first, so there are no
+//   more groups than in an aligned row (with one more, 16384 x 1023 bf16 rows took
+//   31.6 us: a warp for one group).
+// - The copy takes the units that the row touches; what belongs to the rows next to it
+//   is not used. Elements of 16-byte units that reach out of the tensor are added by
+//   the threads.
+// - An x, or an up half, that lies otherwise than the groups is moved into place in
+//   registers. A residual that lies otherwise than x is read an element at a time, and
+//   so a norm's q is written where it lies otherwise than x.
 constexpr int kMaxDepth = 8;
 constexpr int kStreamThreads = 512;
 
 __device__ __forceinline__ uintptr_t down16(uintptr_t p) { return p & ~(uintptr_t)15; }
 __device__ __forceinline__ uintptr_t up16(uintptr_t p) { return (p + 15) & ~(uintptr_t)15; }
 
-// One input of a ragged row: where its bytes are and which of them are copied.
-struct RaggedRow
+// Elements [pos, pos + 8) at p, where p + pos - shift is a unit of 8 elements (shift: 0
+// to 7, the same in every thread): aligned 16-byte loads, moved into place by selects
+// (a switch over the shift was 5 to 15 % slower). CHECK: loads that begin outside
+// [0, end) are left out.
+template <typename T, bool CHECK>
+__device__ __forceinline__ Raw8<T> load8_shifted(const uint8_t *p, int pos, int shift, int end)
 {
-    uintptr_t begin, lo, hi; // the row's first byte; the copied bytes [lo, hi)
-    bool clipped;            // some of its units reach out of the tensor
-    __device__ __forceinline__ RaggedRow(const void *base, int64_t row, int64_t row_bytes, int64_t n_rows)
+    constexpr int kVec = 16 / sizeof(T), kLoads = 8 / kVec + 1, kWords = 8 * sizeof(T) / 4;
+    shift %= kVec;
+    const int first = pos - shift;
+    if (!CHECK && shift == 0)
+        return load8_shared<T>(p + first * (int)sizeof(T));
+    uint32_t w[4 * kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
     {
-        const uintptr_t first = (uintptr_t)base, end = first + n_rows * row_bytes;
-        begin = first + row * row_bytes;
-        lo = down16(begin);
-        hi = up16(begin + row_bytes);
-        clipped = lo < first || hi > end;
-        if (clipped)
-        {
-            lo = lo < first ? up16(first) : lo;
-            hi = hi > end ? down16(end) : hi;
-            hi = hi > lo ? hi : lo;
-        }
+        uint4 v = {};
+        const int e = first + kVec * i;
+        if ((!CHECK || (e >= 0 && e < end)) && (i < kLoads - 1 || shift))
+            v = *reinterpret_cast<const uint4 *>(p + e * (int)sizeof(T));
+        __builtin_memcpy(w + 4 * i, &v, sizeof(v));
     }
-    // Elements `stride` apart from the e-th on, those below `end`; zeros for the rest.
-    template <typename T>
-    __device__ __forceinline__ Raw8<T> load(const uint8_t *stage, int e, int stride, int end) const
-    {
-        const T *p = reinterpret_cast<const T *>(stage + (begin & 15));
-        T v[8];
-        if (!clipped && e + 7 * stride < end)
+    const int by = shift * (int)sizeof(T); // bytes
+#pragma unroll
+    for (int step = 2; step; step /= 2)
+        if (by & (4 * step))
         {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = p[e + i * stride];
+            for (int i = 0; i < kWords + step - 1 + (sizeof(T) == 2); ++i)
+                w[i] = i + step < 4 * kLoads ? w[i + step] : 0;
         }
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-            {
-                const int x = e + i * stride;
-                const uintptr_t g = begin + (int64_t)x * sizeof(T);
-                v[i] = x >= end ? from_f<T>(0.f) : g >= lo && g < hi ? p[x] : *reinterpret_cast<const T *>(g);
-            }
-        }
-        Raw8<T> r;
-        __builtin_memcpy(&r, v, sizeof(r));
-        return r;
-    }
-};
-
-// Values into elements `stride` apart from the e-th on, those below `end`.
-template <typename B>
-__device__ __forceinline__ void scatter8(B *p, const B (&v)[8], int e, int stride, int end)
-{
-    if (e + 7 * stride < end)
+    if (sizeof(T) == 2 && (by & 2))
     {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            p[e + i * stride] = v[i];
+        for (int i = 0; i < kWords; ++i)
+            w[i] = __funnelshift_r(w[i], w[i + 1], 16);
     }
-    else
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (e + i * stride < end)
-                p[e + i * stride] = v[i];
-    }
+    Raw8<T> r;
+    __builtin_memcpy(&r, w, sizeof(r));
+    return r;
 }
 
 // THREADS: the most threads of a launch; below kStreamThreads the instantiation is held
@@ -621,19 +608,88 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
     const void *const base = kNorm ? a.xio : a.x;
     const uint32_t stage_bytes = input_bytes * kCopies;
     const int64_t n_mine = (a.n_rows - blockIdx.x + gridDim.x - 1) / gridDim.x; // (gridDim.x <= n_rows)
+    auto place = [&](const void *tensor) { // of this CTA's rows in their units of 8 elements
+        return RAGGED ? (int)((((uintptr_t)tensor + blockIdx.x * row_bytes) / sizeof(T)) & 7) : 0;
+    };
+    const int off = place(base);
+    const int cut = kNorm ? off : RAGGED ? (int)(((uintptr_t)a.q + blockIdx.x * a.dim) & 7) : 0;
+    const int off2 = SRC == SRC_NORM_ADD ? place(a.residual) : 0;
+    const bool q_aligned = !RAGGED || (((uintptr_t)a.q + blockIdx.x * a.dim - cut) & 7) == 0;
+    const int n_elements = (dim + 7) / 8 * 8; // of all groups
+    auto mine = [&](int j) { return 8 * (j * n_threads + tid) < dim; };
+    // The first element of group j; below 0 in a ragged row's first group, where an
+    // element e < 0 stands for e + n_elements. Thread 0 begins with the last group, so
+    // that the partial ones are its first and thread 1's.
+    auto at = [&](int j) {
+        const int e = 8 * (j * n_threads + tid) - cut;
+        return !RAGGED ? e : j == 0 && tid == 0 ? e + n_elements - 8 : e - 8;
+    };
+    auto partial = [&](int j, int e) { return RAGGED && j == 0 && (e < 0 || e + 8 > dim); };
+    auto element = [&](int e, int i) { return e + i < 0 ? e + i + n_elements : e + i; }; // (in the row if < dim)
+    auto gather = [&](const T *p, int e) {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = element(e, i) < dim ? p[element(e, i)] : from_f<T>(0.f);
+        Raw8<T> r;
+        __builtin_memcpy(&r, v, sizeof(r));
+        return r;
+    };
+    // A partial group: `own` as it lies, with the elements before the row from `last`.
+    auto join = [&](int e, const Raw8<T> &own, const Raw8<T> &last) {
+        T v[8], l[8];
+        unpack8(own, v);
+        unpack8(last, l);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            v[i] = e + i < 0 ? l[i] : v[i];
+            v[i] = element(e, i) < dim ? v[i] : from_f<T>(0.f);
+        }
+        Raw8<T> r;
+        __builtin_memcpy(&r, v, sizeof(r));
+        return r;
+    };
+    constexpr uint32_t kUnit = 8 * sizeof(T);
+    auto unit_bytes = [&](int c) { return ((uint32_t)row_bytes + c * (uint32_t)sizeof(T) + kUnit - 1) / kUnit * kUnit; };
+    const int n_end = dim >= 8 ? 1 : 8; // rows at each end of the tensor whose units may reach out
+    auto at_end = [&](int64_t row) { return row < n_end || row >= a.n_rows - n_end; };
+    // Bytes [at, at + n) of the n of a row's units at p are in the tensor's whole 16-byte units.
+    auto clip = [&](const void *tensor, const uint8_t *p, uint32_t &at, uint32_t &n) {
+        const uintptr_t first = up16((uintptr_t)tensor), end = down16((uintptr_t)tensor + a.n_rows * row_bytes);
+        const uintptr_t lo = (uintptr_t)p < (uintptr_t)tensor ? first : (uintptr_t)p;
+        const uintptr_t hi = (uintptr_t)p + n < end ? (uintptr_t)p + n : end;
+        at = (uint32_t)(lo - (uintptr_t)p);
+        n = hi > lo ? (uint32_t)(hi - lo) : 0;
+    };
+    // Elements that clip leaves out, from global memory.
+    auto complete = [&](const void *tensor, int64_t row, int c, uint8_t *stage) {
+        const T *src = reinterpret_cast<const T *>(static_cast<const uint8_t *>(tensor) + row * row_bytes);
+        uint32_t at = 0, n = unit_bytes(c);
+        clip(tensor, reinterpret_cast<const uint8_t *>(src - c), at, n);
+        for (int e = tid; e < (int)(row_bytes / (int)sizeof(T)); e += n_threads)
+            if ((uint32_t)(c + e) * sizeof(T) < at || (uint32_t)(c + e) * sizeof(T) >= at + n)
+                reinterpret_cast<T *>(stage)[c + e] = src[e];
+    };
     auto issue = [&](int64_t it, int slot) {
         const int64_t row = blockIdx.x + it * gridDim.x;
         const uint32_t dst = smem_u32(ring) + slot * stage_bytes, bar = smem_u32(&s_full[slot]);
         if constexpr (RAGGED)
         {
-            const RaggedRow x(base, row, row_bytes, a.n_rows);
-            const RaggedRow r(kCopies == 2 ? a.residual : base, row, row_bytes, a.n_rows);
-            const uint32_t nx = (uint32_t)(x.hi - x.lo), nr = kCopies == 2 ? (uint32_t)(r.hi - r.lo) : 0;
+            const uint8_t *x = static_cast<const uint8_t *>(base) + row * row_bytes - off * (int)sizeof(T);
+            const uint8_t *r = static_cast<const uint8_t *>(a.residual) + row * row_bytes - off2 * (int)sizeof(T);
+            uint32_t at_x = 0, at_r = 0, nx = unit_bytes(off), nr = kCopies == 2 ? unit_bytes(off2) : 0;
+            if (at_end(row))
+            {
+                clip(base, x, at_x, nx);
+                if (kCopies == 2)
+                    clip(a.residual, r, at_r, nr);
+            }
             mbar_expect_tx(bar, nx + nr);
             if (nx)
-                bulk_load(dst + (uint32_t)(x.lo - down16(x.begin)), (const void *)x.lo, nx, bar);
+                bulk_load(dst + at_x, x + at_x, nx, bar);
             if (nr)
-                bulk_load(dst + input_bytes + (uint32_t)(r.lo - down16(r.begin)), (const void *)r.lo, nr, bar);
+                bulk_load(dst + input_bytes + at_r, r + at_r, nr, bar);
         }
         else
         {
@@ -656,25 +712,24 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
             issue(i, i);
     }
     pdl_wait();
-    // the first element of group j, whose elements are `stride` apart
-    const int stride = RAGGED ? n_threads : 1;
-    auto at = [&](int j) { return RAGGED ? 8 * j * n_threads + tid : 8 * (j * n_threads + tid); };
     Raw8<T> w[NV];
     if (kNorm)
     {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
         {
+            if (!mine(j))
+                continue;
+            const T *from = static_cast<const T *>(a.w);
             if constexpr (RAGGED)
             {
-                T v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = at(j) + i * stride < dim ? static_cast<const T *>(a.w)[at(j) + i * stride] : from_f<T>(0.f);
-                __builtin_memcpy(&w[j], v, sizeof(v));
+                const int e = at(j), shift = (int)(((uintptr_t)from / sizeof(T) - cut) & 7), first = e - shift;
+                w[j] = first >= 0 && first + 16 <= dim
+                           ? load8_shifted<T, false>(reinterpret_cast<const uint8_t *>(from), e, shift, dim)
+                           : gather(from, e);
             }
-            else if (at(j) < dim)
-                w[j] = load8(static_cast<const T *>(a.w) + at(j), true);
+            else
+                w[j] = load8(from + at(j), true);
         }
     }
     __syncthreads();
@@ -692,32 +747,74 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
             s_abort = 1;
         }
         const bool arrived = !*abort_flag; // (a row that has not arrived is not written back)
-        const uint8_t *stage = ring + slot * stage_bytes;
+        uint8_t *stage = ring + slot * stage_bytes;
         Held<T, SRC, NV> held[NV];
         Top<V> top;
         float sq = 0.f;
         if constexpr (RAGGED)
         {
-            const RaggedRow x(base, row, row_bytes, a.n_rows);
-            const RaggedRow r(kCopies == 2 ? a.residual : base, row, row_bytes, a.n_rows);
+            if (at_end(row))
+            {
+                if (arrived)
+                {
+                    complete(base, row, off, stage);
+                    if (kCopies == 2)
+                        complete(a.residual, row, off2, stage + input_bytes);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // (the slot is copied to again)
+                __syncthreads();
+            }
             T *out = static_cast<T *>(a.xio) + row * a.dim;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
             {
-                const int e = at(j);
-                if (e >= dim)
+                int e = at(j);
+                asm volatile("" : "+r"(e)); // (addresses are not held over the rows)
+                if (!mine(j))
                     continue;
-                Raw8<T> in = x.template load<T>(stage, e, stride, dim), in2;
+                const int end = off + dim * (SRC == SRC_SWIGLU ? 2 : 1), shift = kNorm ? 0 : (off - cut) & 7;
+                auto load = [&](auto check, int pos, int shift) {
+                    return load8_shifted<T, decltype(check)::value>(stage, pos, shift, end);
+                };
+                Raw8<T> in, in2;
+                if (!partial(j, e))
+                {
+                    in = load(std::false_type(), off + e, shift);
+                    if (SRC == SRC_SWIGLU)
+                        in2 = load(std::false_type(), off + dim + e, (shift + dim) & 7);
+                }
+                else
+                {
+                    const std::true_type check;
+                    const int last = e + n_elements;
+                    const bool wraps = e < 0 && last < dim;
+                    in = load(check, off + e, shift);
+                    in = join(e, in, wraps ? load(check, off + last, shift) : in);
+                    if (SRC == SRC_SWIGLU)
+                    {
+                        in2 = load(check, off + dim + e, (shift + dim) & 7);
+                        in2 = join(e, in2, wraps ? load(check, off + dim + last, (shift + dim) & 7) : in2);
+                    }
+                }
                 if (SRC == SRC_NORM_ADD)
-                    in2 = r.template load<T>(stage + input_bytes, e, stride, dim);
-                if (SRC == SRC_SWIGLU)
-                    in2 = x.template load<T>(stage, e + dim, stride, 2 * dim);
-                held[j].look(in, in2, w[j], top, sq); // (the zeros past the row add nothing)
+                {
+                    const T *p = reinterpret_cast<const T *>(stage + input_bytes) + off2;
+                    in2 = off2 == off && !partial(j, e) ? load8_shared<T>(reinterpret_cast<const uint8_t *>(p + e)) : gather(p, e);
+                }
+                held[j].look(in, in2, w[j], top, sq); // (zeros beside the row add nothing)
                 if (SRC == SRC_NORM_ADD && arrived)
                 {
-                    T v[8];
-                    unpack8(held[j].in, v);
-                    scatter8(out, v, e, stride, dim);
+                    if (!partial(j, e))
+                        store8(out + e, held[j].in);
+                    else
+                    {
+                        T v[8];
+                        unpack8(held[j].in, v);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (element(e, i) < dim)
+                                out[element(e, i)] = v[i];
+                    }
                 }
             }
         }
@@ -727,7 +824,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
             for (int j = 0; j < NV; ++j)
             {
                 const int e = at(j);
-                if (e >= dim)
+                if (!mine(j))
                     continue;
                 const uint8_t *p = stage + (uint32_t)e * sizeof(T);
                 Raw8<T> in = load8_shared<T>(p), in2;
@@ -751,19 +848,21 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
         {
-            if (at(j) >= dim)
+            if (!mine(j))
                 continue;
             const uint2 b = held[j].quantized(w[j], z);
-            if constexpr (RAGGED)
+            int e = at(j);
+            if (RAGGED)
+                asm volatile("" : "+r"(e));
+            if (q_aligned && !partial(j, e))
+                *reinterpret_cast<uint2 *>(q + e) = b;
+            else
             {
-                int8_t v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    v[i] = (int8_t)((i < 4 ? b.x : b.y) >> (8 * (i & 3)));
-                scatter8(q, v, at(j), stride, dim);
+                    if (element(e, i) < dim)
+                        q[element(e, i)] = (int8_t)((i < 4 ? b.x : b.y) >> (8 * (i & 3)));
             }
-            else
-                *reinterpret_cast<uint2 *>(q + at(j)) = b;
         }
         if (tid == 0)
             a.scales[row] = z.scale;
@@ -883,7 +982,8 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemPerSM));
     if (st != L2K_OK)
         return st;
-    const int64_t grid = std::min<int64_t>(a.n_rows, per_sm * num_sms());
+    const int64_t most = per_sm * num_sms();
+    const int64_t grid = std::min<int64_t>(a.n_rows, RAGGED ? std::max<int64_t>(8, most / 8 * 8) : most);
     return launch_pdl(kernel, (unsigned)grid, threads, (size_t)(depth * stage_bytes), stream, a, depth, (uint32_t)input_bytes);
 }
 
@@ -895,7 +995,9 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
 // rows; more where the row needs it. CTAs of 352 to 448 threads would leave an SM
 // one of them at the 86 to 96 registers of the plain instantiation: 4099 x 13824 f16
 // SwiGLU 75 us, 56 with two; 8192 x 11008 bf16 rows 74, 55 with two; likewise fp32
-// norms of 288 to 320 threads (8192 x 5120: 114 us, 100 with two). 16-bit norms stay at
+// norms of 288 to 320 threads (8192 x 5120: 114 us, 100 with two), and fp32 ragged rows
+// of any length (16384 x 4095 SwiGLU 230 us at 115 registers, 116 at 72; 16-bit ones
+// without gain: 16384 x 1023 rows 29 us, 19 without). 16-bit norms stay at
 // their 122 to 126: held to 80 they spill (16384 x 4096: 94 us against 76).
 template <typename T, int SRC, bool RAGGED>
 int launch_stream(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes, cudaStream_t stream)
@@ -906,14 +1008,15 @@ int launch_stream(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes, cu
     const int want = groups <= 32 || (kWide && SRC == SRC_SWIGLU) || (RAGGED && few) ? 1
                      : kWide || groups <= 64 || (few && !kNorm)                      ? 2
                                                                                      : 4;
-    if (want == 1 && groups <= kStreamThreads)
-        return launch_stream_nv<T, SRC, 1, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
-    if constexpr (kNorm && kWide && !RAGGED)
+    constexpr int kMost = RAGGED && !kNorm && kWide ? 448 : kStreamThreads;
+    if (want == 1 && groups <= kMost)
+        return launch_stream_nv<T, SRC, 1, RAGGED, kMost>(a, input_bytes, stage_bytes, stream);
+    if constexpr (kNorm && kWide)
         if (groups > 2 * 256 && groups <= 2 * 320)
             return launch_stream_nv<T, SRC, 2, RAGGED, 320>(a, input_bytes, stage_bytes, stream);
-    if (want <= 2 && groups <= 2 * kStreamThreads)
-        return launch_stream_nv<T, SRC, 2, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
-    if constexpr (!kNorm && !RAGGED)
+    if (want <= 2 && groups <= 2 * kMost)
+        return launch_stream_nv<T, SRC, 2, RAGGED, kMost>(a, input_bytes, stage_bytes, stream);
+    if constexpr (!kNorm)
         if (groups > 4 * 320 && groups <= 4 * 448)
             return launch_stream_nv<T, SRC, 4, RAGGED, 448>(a, input_bytes, stage_bytes, stream);
     return launch_stream_nv<T, SRC, 4, RAGGED, kStreamThreads>(a, input_bytes, stage_bytes, stream);
@@ -924,9 +1027,11 @@ int launch_rows(const RowArgs &a, const char *name, cudaStream_t stream)
 {
     const bool vec = a.dim % 8 == 0 && is_aligned(a.x, 16) && is_aligned(a.xio, 16) && is_aligned(a.residual, 16) &&
                      is_aligned(a.w, 16) && is_aligned(a.q, 8);
+    constexpr int64_t kUnit = 8 * sizeof(T);
     const int64_t groups = ceil_div(a.dim, 8);
     const int64_t row_bytes = a.dim * (SRC == SRC_SWIGLU ? 2 : 1) * (int64_t)sizeof(T);
-    const int64_t input_bytes = vec ? row_bytes : (row_bytes + 30) / 16 * 16; // (the 16-byte units a row touches)
+    // (without alignment: the units of 8 elements that a row touches)
+    const int64_t input_bytes = vec ? row_bytes : (row_bytes + 7 * (int64_t)sizeof(T) + kUnit - 1) / kUnit * kUnit;
     const int64_t stage_bytes = input_bytes * (SRC == SRC_NORM_ADD ? 2 : 1);
     const bool stream_fits = groups <= 4 * kStreamThreads && stage_bytes <= kSmemPerSM;
     int st = L2K_OK;

@@ -227,6 +227,33 @@ def test_swiglu_of_any_alignment(dtype, shift):
     _check_swiglu(x, 5, 520, shift)
 
 
+# (rows, length): several rows a CTA at each distance of a row from a multiple of 8
+# elements, rows shorter than 8 elements, whole tensors inside one 16-byte unit
+RAGGED = [(5000, 263), (3001, 257), (2403, 1020), (4000, 5), (1, 3), (17, 1), (700, 14)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("at", [(0, 0, 0, 0), (1, 1, 1, 1), (3, 5, 2, 7), (8, 4, 1, 2)])
+@pytest.mark.parametrize("n,dim", RAGGED)
+def test_rows_and_outputs_placed_apart(n, dim, at, dtype):
+    """x, the residual, the weights and q each at an alignment of its own."""
+    x = placed(torch.randn(n, dim, generator=gen(1), device="cuda").to(dtype), at[0])
+    q, s, qs, ss = row_outputs(n, dim, at[3])
+    ops.launch_quantize_rows_int8(x, q, s)
+    want, scale = reference_rows(x.double())
+    assert torch.equal(q.double(), want)
+    check_scales(s, scale, U)
+    check_untouched(n, dim, at[3], qs, ss)
+
+    r = placed(torch.randn(n, dim, generator=gen(2), device="cuda").to(dtype), at[1])
+    w = placed((torch.rand(dim, generator=gen(3), device="cuda") + 0.5).to(dtype), at[2])
+    before = x._base[:at[0]].fill_(SENTINEL)
+    _check_norm(x, r, w, False, at[3])
+    _check_norm(x, r, w, True, at[3])
+    assert (before == SENTINEL).all()
+    _check_swiglu(placed(torch.randn(n, 2 * dim, generator=gen(4), device="cuda").to(dtype), at[0]), n, dim, at[3])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_swiglu_special_rows(dtype):
     dim = 128

@@ -353,15 +353,57 @@ __device__ __forceinline__ void unpack8(const Raw8<T> &r, T (&v)[8])
     __builtin_memcpy(v, &r, sizeof(r));
 }
 
+template <typename T>
+__device__ __forceinline__ float2 pair(const T (&v)[8], int e)
+{
+    return make_float2(to_f(v[e]), to_f(v[e + 1]));
+}
+
+// The largest magnitude of 16-bit values, two at a time (the sign that the instruction
+// gives is not used): 16384 x 4096 bf16 rows 38 us, 41 through fp32. Packed additions
+// and products in the norms, a fifth fewer instructions, were not kept: 8192 x 11008 111
+// us against 125, but 16384 x 4096 88 against 76, launches back to back.
+template <typename T>
+struct TopPacked
+{
+    using Bits = uint32_t;
+    uint32_t v = 0;
+    __device__ __forceinline__ void add(const Raw8<T> &r)
+    {
+#pragma unroll
+        for (uint32_t x : {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w})
+            if constexpr (std::is_same<T, __half>::value)
+                asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(v) : "r"(x));
+            else
+                asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(x));
+    }
+    __device__ __forceinline__ Bits bits() const
+    {
+        T e[2];
+        __builtin_memcpy(e, &v, sizeof(e));
+        TopF top;
+        top.add(to_f(e[0]), to_f(e[1]));
+        return top.bits();
+    }
+};
+
 // silu(g) * u in fp32 by the fast exponential and reciprocal, for every type: their
 // errors (2 + 1.2 |g| steps of fp32 and 1) are 1e-6 of an 8-bit row's step. 0
 // where exp(-g) leaves the range of fp32 (g < -87), as in l2k_swiglu.
+__device__ __forceinline__ float2 silu_up2(float2 g, float2 u)
+{
+    const float2 x = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+    const float2 d = add2(e, make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+    return mul2(mul2(g, r), u);
+}
 __device__ __forceinline__ float silu_up(float g, float u)
 {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(e, 1.0f)));
-    return __fmul_rn(__fmul_rn(g, r), u);
+    return silu_up2(make_float2(g, g), make_float2(u, u)).x;
 }
 
 // y of 8 elements of a row (or with ADD of the sum to write back) and the norm's weights.
@@ -385,28 +427,35 @@ struct Held
 {
     using V = typename RowValue<T, SRC>::type;
     static constexpr bool kNorm = SRC == SRC_NORM || SRC == SRC_NORM_ADD;
+    static constexpr bool kPacked = SRC == SRC_ROWS && sizeof(T) == 2;
+    using RowTop = std::conditional_t<kPacked, TopPacked<T>, Top<V>>;
     static constexpr bool kKeep = SRC == SRC_SWIGLU || (sizeof(V) == 8 && NV <= 2);
     Raw8<T> in;
     V y[8];
 
     // The first look: in2 is the residual, or SwiGLU's up half; with ADD `in`
     // becomes the sum to write back.
-    __device__ __forceinline__ void look(const Raw8<T> &first, const Raw8<T> &in2, const Raw8<T> &w, Top<V> &top, float &sq)
+    __device__ __forceinline__ void look(const Raw8<T> &first, const Raw8<T> &in2, const Raw8<T> &w, RowTop &top, float &sq)
     {
         T v[8], u[8];
-        unpack8(first, v);
         if constexpr (SRC == SRC_SWIGLU)
         {
+            unpack8(first, v);
             unpack8(in2, u);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                y[e] = silu_up(to_f(v[e]), to_f(u[e]));
+            for (int e = 0; e < 8; e += 2)
+            {
+                const float2 t = silu_up2(pair(v, e), pair(u, e));
+                y[e] = t.x;
+                y[e + 1] = t.y;
+            }
 #pragma unroll
             for (int e = 0; e < 8; e += 2)
                 top.add(y[e], y[e + 1]);
         }
         else
         {
+            unpack8(first, v);
             if constexpr (SRC == SRC_NORM_ADD)
             {
                 unpack8(in2, u);
@@ -421,15 +470,20 @@ struct Held
                 for (int e = 0; e < 8; ++e)
                     sq = fmaf(to_f(v[e]), to_f(v[e]), sq);
             }
-            V t[8];
-            values8<T, SRC>(in, w, t);
+            if constexpr (kPacked)
+                top.add(in);
+            else
+            {
+                V t[8];
+                values8<T, SRC>(in, w, t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (kKeep)
-                    y[e] = t[e];
+                for (int e = 0; e < 8; ++e)
+                    if (kKeep)
+                        y[e] = t[e];
 #pragma unroll
-            for (int e = 0; e < 8; e += 2)
-                top.add(t[e], t[e + 1]);
+                for (int e = 0; e < 8; e += 2)
+                    top.add(t[e], t[e + 1]);
+            }
         }
     }
     __device__ __forceinline__ uint2 quantized(const Raw8<T> &w, const Quantizer<V> &z) const
@@ -485,7 +539,7 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_kernel(const RowArgs a)
         }
     }
     Held<T, SRC, NV> held[NV];
-    Top<V> top;
+    typename Held<T, SRC, NV>::RowTop top;
     float sq = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -749,7 +803,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
         const bool arrived = !*abort_flag; // (a row that has not arrived is not written back)
         uint8_t *stage = ring + slot * stage_bytes;
         Held<T, SRC, NV> held[NV];
-        Top<V> top;
+        typename Held<T, SRC, NV>::RowTop top;
         float sq = 0.f;
         if constexpr (RAGGED)
         {
@@ -989,7 +1043,7 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
 
 // Groups per thread: one for the shortest rows (a warp or less); four for 16-bit
 // rows (the reduction's fixed cost of about 60 instructions a warp is shared by
-// four groups: 16384 x 4096 bf16 rows 40 us, 44 with two), two where a few rows per
+// four groups: 16384 x 4096 bf16 rows 40 us, 44 with two, eight no faster), two where a few rows per
 // SM leave threads idle (512 rows: 4.0 us, 4.7 with one); two for fp32 rows (53 us,
 // 60 with four) and one for fp32 SwiGLU (90 us, 99 with two) and a few ragged
 // rows; more where the row needs it. CTAs of 352 to 448 threads would leave an SM

@@ -582,7 +582,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 // Aligned rows (16-byte aligned, a multiple of 8 elements): 16-byte accesses.
 // RAGGED: rows of any length and alignment, in 16-byte accesses too (an element at a
 // time, 16384 x 1023 bf16 rows took 25 us, norms 61, SwiGLU 41; now 20, 39, 32; 4099 x
-// 13799: 82, 197, 126, now 46, 114, 85):
+// 13799: 82, 197, 126, now 44, 114, 85):
 // - A CTA's rows lie a multiple of 8 rows apart, so all of them lie alike with respect
 //   to the units of 8 elements in memory.
 // - The groups are cut where q's bytes (norms: the row that is written back) can be

@@ -85,6 +85,7 @@ struct alignas(16) Vec16
 // 16-byte global accesses.
 //   ldg_stream: read-only, do not allocate in L1 (data read once).
 //   ldg_keep:   read-only through the non-coherent path (reused data).
+//   ldg_coherent[_u32, _f32]: data that another kernel may write while this one runs.
 //   stg_stream: streaming store (evict-first).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint4 ldg_stream(const void *p)
@@ -109,6 +110,18 @@ __device__ __forceinline__ uint4 ldg_coherent(const void *p)
     asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                  : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint32_t ldg_coherent_u32(const uint32_t *p)
+{
+    uint32_t r;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ float ldg_coherent_f32(const float *p)
+{
+    float r;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(r) : "l"(p));
     return r;
 }
 __device__ __forceinline__ void stg_stream(void *p, uint4 v)
@@ -164,8 +177,11 @@ __device__ __forceinline__ float silu_mul(float g, float u)
 // while the kernel before it in the stream ends. It touches no global memory before
 // pdl_wait(), which returns once that kernel has completed and its writes are
 // visible; what comes before (barriers, tensor memory, instruction fetch) overlaps
-// the other's end. pdl_trigger() lets the next such kernel start once every CTA of
-// this one has called it or left.
+// the other's end. What it then reads may have been written while it was running, so
+// it reads through the coherent path (ldg_coherent, plain loads or bulk copies; a
+// __ldg could be moved above the wait or answered by a line that an earlier kernel
+// left in L1). pdl_trigger() lets the next such kernel start once every CTA of this
+// one has called it or left.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -265,7 +265,7 @@ __device__ __forceinline__ uint4 load_unaligned16(const int8_t *p, int64_t valid
         uint32_t x[5];
 #pragma unroll
         for (int i = 0; i < 5; ++i)
-            x[i] = __ldg(w + i);
+            x[i] = ldg_coherent_u32(w + i);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     {
         pdl_wait();
         for (int i = tid - 9 * 32; i < bn; i += kTThreads - 9 * 32)
-            sb[i] = col0 + i < a.n ? __ldg(a.sb + col0 + i) : 0.f;
+            sb[i] = col0 + i < a.n ? ldg_coherent_f32(a.sb + col0 + i) : 0.f;
     }
     pdl_wait(); // (every thread: the epilogue reads scales and writes C)
     tc_fence_before();
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     const int quad = warp & 3, part = warp >> 2;
     const int lrow = BM == 64 ? 16 * quad + lane : 32 * quad + lane;
     const bool live = (BM == 128 || lane < 16) && row0 + lrow < a.m;
-    const float row_scale = live ? __ldg(a.sa + row0 + lrow) : 0.f;
+    const float row_scale = live ? ldg_coherent_f32(a.sa + row0 + lrow) : 0.f;
     if (!mbar_wait(bar_done, 0, abort_flag))
         int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
     if (*abort_flag && warp < groups && lane == 0)
@@ -592,8 +592,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 uint32_t r[8];
                 *reinterpret_cast<int4 *>(r) = *reinterpret_cast<const int4 *>(stage + rr * stride + c);
                 *reinterpret_cast<int4 *>(r + 4) = *reinterpret_cast<const int4 *>(stage + rr * stride + c + 4);
-                store8<T>(static_cast<T *>(a.c) + (row0 + rr) * a.ldc + col0 + c, r, __ldg(a.sa + row0 + rr), sb + c,
-                          a.n - col0 - c, a.wide);
+                store8<T>(static_cast<T *>(a.c) + (row0 + rr) * a.ldc + col0 + c, r,
+                          ldg_coherent_f32(a.sa + row0 + rr), sb + c, a.n - col0 - c, a.wide);
             }
         __syncwarp();
         cluster_barrier_relaxed(); // no rank leaves while another may still read its partial
@@ -825,11 +825,11 @@ __global__ void __launch_bounds__(kPThreads, 1)
             const TileAt t = tile_at(tile, m_tiles, a.n_nt);
             const int64_t row = t.row * 256 + 128 * (int64_t)rank + 32 * quad + lane, col0 = t.col * 256 + 128 * part;
             const bool store = row < a.m;
-            const float row_scale = store ? __ldg(a.sa + row) : 0.f;
+            const float row_scale = store ? ldg_coherent_f32(a.sa + row) : 0.f;
             float sb[4]; // the scales of this warp's columns 32 i + lane
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                sb[i] = col0 + 32 * i + lane < a.n ? __ldg(a.sb + col0 + 32 * i + lane) : 0.f;
+                sb[i] = col0 + 32 * i + lane < a.n ? ldg_coherent_f32(a.sb + col0 + 32 * i + lane) : 0.f;
             if (!mbar_wait(bar_acc_full + 8 * buf, (uint32_t)(lt >> 1) & 1u, abort_flag))
             {
                 int8_fail(ERR_INT8_WAIT_DONE, abort_flag);

@@ -315,12 +315,12 @@ struct Raw8
     uint4 v[sizeof(T) / 2];
 };
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T *p, bool keep)
+__device__ __forceinline__ Raw8<T> load8(const T *p)
 {
     Raw8<T> r;
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-        r.v[i] = keep ? ldg_keep(p + 16 / sizeof(T) * i) : ldg_coherent(p + 16 / sizeof(T) * i);
+        r.v[i] = ldg_coherent(p + 16 / sizeof(T) * i);
     return r;
 }
 template <typename T>
@@ -529,13 +529,13 @@ __global__ void __launch_bounds__(kMaxThreads) rows_int8_kernel(const RowArgs a)
         const int g = threadIdx.x + j * blockDim.x;
         if (g < n_groups)
         {
-            in[j] = load8(src + 8 * g, false);
+            in[j] = load8(src + 8 * g);
             if (SRC == SRC_NORM_ADD)
-                in2[j] = load8(add + 8 * g, false);
+                in2[j] = load8(add + 8 * g);
             if (SRC == SRC_SWIGLU)
-                in2[j] = load8(src + a.dim + 8 * g, false);
+                in2[j] = load8(src + a.dim + 8 * g);
             if (kNorm)
-                w[j] = load8(static_cast<const T *>(a.w) + 8 * g, true);
+                w[j] = load8(static_cast<const T *>(a.w) + 8 * g);
         }
     }
     Held<T, SRC, NV> held[NV];
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < kStreamThreads ? 2 : 1)
                            : gather(from, e);
             }
             else
-                w[j] = load8(from + at(j), true);
+                w[j] = load8(from + at(j));
         }
     }
     __syncthreads();

@@ -111,6 +111,13 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank)
     return r;
 }
 
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
+{
+    uint32_t r;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(r) : "r"(addr) : "memory");
+    return r;
+}
+
 // 16 consecutive accumulator columns of this thread's TMEM lane (no wait).
 __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16])
 {
@@ -210,7 +217,9 @@ __device__ __forceinline__ T staged(const uint8_t *staging, int row, int col)
 // drained ring). After a cluster barrier each rank adds its rows [q rows_per,
 // (q + 1) rows_per) into rank q's copy with one bulk reduction, and rank q
 // scales and stores those rows once all have landed. A last barrier keeps every
-// copy alive until it has been read.
+// copy alive until it has been read. A rank that has failed takes the same steps, so
+// that every reduction lands before its CTAs leave; each rank reads the others' failure
+// flags while the reductions are on their way, and stores nothing if one is set.
 //
 // The A box has a.a_rows rows (m rounded up to 8). The MMA reads BM: the rest is
 // whatever follows in shared memory (a stage lies BM rows from its end at the
@@ -303,9 +312,10 @@ __global__ void __launch_bounds__(kTThreads, 1)
     const uint32_t bar_full = sbase + a.ring_bytes + 4 * bn; // + 8 * stage: the stage's tiles landed
     const uint32_t bar_freed = bar_full + 8 * kTMaxStages;   // + 8 * stage: the MMAs reading it completed
     const uint32_t bar_done = bar_freed + 8 * kTMaxStages;   // every group's MMAs completed
-    const uint32_t bar_red = bar_done + 8;                   // the other ranks' rows have been added
+    const uint32_t bar_red = bar_done + 8;                   // the other ranks' rows have been added, their flags read
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + a.ring_bytes + 4 * bn + 8 * (2 * kTMaxStages + 2));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const uint32_t abort_addr = smem_u32(tmem_slot + 1);
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0); // (uniform, known as such)
@@ -354,7 +364,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         if (elect_one())
         {
             mbar_init(bar_done, groups);
-            mbar_init(bar_red, 1);
+            mbar_init(bar_red, split);
             *abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -574,14 +584,21 @@ __global__ void __launch_bounds__(kTThreads, 1)
             mbar_expect_tx(bar_red, (uint32_t)((split - 1) * mine * stride * 4));
         __syncwarp();
         cluster_barrier(); // every rank's partial is in its shared memory
-        if (warp < split && warp != rank && rows_of(warp) > 0 && elect_one())
+        if (warp < split && warp != rank && elect_one())
         {
-            const uint32_t src = sbase + (uint32_t)(warp * rows_per * stride) * 4;
-            bulk_add_s32(cluster_addr(src, (uint32_t)warp), src, (uint32_t)(rows_of(warp) * stride * 4),
-                         cluster_addr(bar_red, (uint32_t)warp));
+            if (rows_of(warp) > 0)
+            {
+                const uint32_t src = sbase + (uint32_t)(warp * rows_per * stride) * 4;
+                bulk_add_s32(cluster_addr(src, (uint32_t)warp), src, (uint32_t)(rows_of(warp) * stride * 4),
+                             cluster_addr(bar_red, (uint32_t)warp));
+            }
+            if (ld_cluster_u32(cluster_addr(abort_addr, (uint32_t)warp)) != 0) // (its partial is incomplete)
+                *abort_flag = 1;
+            mbar_arrive(bar_red);
         }
         __syncwarp();
-        if (mine > 0 && !mbar_wait(bar_red, 0, abort_flag))
+        const int quiet = 0; // (after a failure too: what is being added here lands first)
+        if (mine > 0 && !mbar_wait(bar_red, 0, &quiet))
             int8_fail(ERR_INT8_WAIT_DONE, abort_flag);
         // this rank's rows in runs of 8 columns; a warp's lanes take neighbouring runs
         const int runs = bn / 8, items = runs * mine;

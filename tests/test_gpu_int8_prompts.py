@@ -27,6 +27,7 @@ def _lib(cuda_lib):
 
 # aligned
 ALIGNED = [(3000, 256),     # one group to a thread, one warp to a CTA
+           (800, 512),      # 64 groups: two to a thread
            (500, 1024),     # two groups of few rows
            (2500, 520),     # 65 groups: the first length with four groups to a thread of 16 bits
            (2500, 4096),    # four groups (fp32: two)

@@ -614,10 +614,12 @@ int l2k_decode_step_no_alloc(const l2k_decode_step_args *args, l2k_stream_t stre
  * (ties to even; q does not depend on the order of any sum). A row of zeros,
  * or without elements, has q = 0 and scale 0; a row that holds a NaN or an
  * infinity has q = 0 and scale NaN, so every product of it is NaN. All tensors
- * are row-major and contiguous except the operands of l2k_linear_int8, which
- * have row strides. 16-byte aligned tensors with rows of a multiple of 8
- * elements (16 bytes for l2k_linear_int8's operands) run fastest; any other
- * alignment and length works.
+ * are row-major and contiguous except those of l2k_linear_int8, which has row
+ * strides for a, b and c. Any length and any alignment to elements works. The row
+ * operators run fastest on 16-byte aligned tensors with rows of a multiple of 8
+ * elements, up to 16384 of them: other rows take up to 1.7 times as long, longer
+ * ones 2 to 5 times. l2k_linear_int8 runs fastest on operands whose bases and row
+ * strides are multiples of 16 bytes: others take 4 to 12 times as long.
  *
  * l2k_quantize_rows_int8: y = x, x (num_rows, dim), q (num_rows, dim),
  *   scales (num_rows). For the attention output before the O projection, and
@@ -627,7 +629,9 @@ int l2k_decode_step_no_alloc(const l2k_decode_step_args *args, l2k_stream_t stre
  *   to x, rounded to dtype); y = x * weights / sqrt(mean(x^2) + 1e-5), not
  *   rounded to dtype. residual is read only (may be NULL without
  *   add_residual). As in that operator the squares are summed in fp32: a row
- *   whose sum leaves its range has 1/rms 0, here scale 0.
+ *   whose sum leaves its range has 1/rms 0, here scale 0. x * weights is formed
+ *   in fp32 for 16-bit types (exactly, between 2^-133 and 2^128) and in fp64 for
+ *   fp32; a bf16 row with a product beyond 2^128 counts as holding an infinity.
  * l2k_swiglu_int8: l2k_swiglu with the output row as int8, y in fp32 not
  *   rounded to dtype. The exponential and the reciprocal are the fast ones for
  *   every type (l2k_swiglu's are exact to a step or two for fp32): y is off by

@@ -180,7 +180,7 @@ __device__ __noinline__ uint32_t quantize_divided(float y, float a)
 // both less p, the second one's fp64 value, which leaves a few bits of either next to
 // the border, and the sign in any case. k is the quotient in fp32, rounded down; next
 // to an integer either neighbour leads to the same result. (An fp64 division here took
-// registers from the callers: 8192 x 5120 fp32 norms 107 us.)
+// registers from the callers: 8192 x 5120 fp32 norms 107 us, 95 without.)
 __device__ __noinline__ uint32_t quantize_divided(double y, double a)
 {
     const double m = fabs(y), unit = __hiloint2double(0x7fe00000 - (__double2hiint(a) & 0x7ff00000), 0); // a unit: 1 to 2
@@ -440,7 +440,7 @@ __device__ __forceinline__ void values8(const Raw8<T> &in, const Raw8<T> &w, V (
 }
 
 // What a thread holds of 8 elements from the first look at them to the second:
-// SwiGLU's y, and fp64 products where the registers allow (NV <= 2: 133 us for
+// SwiGLU's y, and fp64 products where the registers allow (NV <= 2: 137 us for
 // 16384 x 4096 fp32 norms, 154 when they are computed twice); else the inputs, half
 // the registers or less, from which y is computed again.
 template <typename T, int SRC, int NV>
@@ -1070,7 +1070,7 @@ int launch_stream_nv(const RowArgs &a, int64_t input_bytes, int64_t stage_bytes,
 // rows; more where the row needs it. CTAs of 352 to 448 threads would leave an SM
 // one of them at the 86 to 96 registers of the plain instantiation: 4099 x 13824 f16
 // SwiGLU 75 us, 56 with two; 8192 x 11008 bf16 rows 74, 55 with two; likewise fp32
-// norms of 288 to 320 threads (8192 x 5120: 114 us, 100 with two), and fp32 ragged rows
+// norms of 288 to 320 threads (8192 x 5120: 114 us, 95 with two), and fp32 ragged rows
 // of any length (16384 x 4095 SwiGLU 230 us at 115 registers, 116 at 72; 16-bit ones
 // without gain: 16384 x 1023 rows 29 us, 19 without). 16-bit norms stay at
 // their 122 to 126: held to 80 they spill (16384 x 4096: 94 us against 76).

@@ -99,3 +99,13 @@ def test_next_to_a_border(n, dim, x0, w0, x1, w1):
     x[:, 2], w[2] = -x0, w0
     check(x, w, [0, n - 1])
     check(placed(x, 1), w, [n - 1])
+
+
+def test_products_past_the_range_of_fp32():
+    """bf16 products x w are formed in fp32: a row with one beyond it counts as holding an infinity."""
+    x = torch.full((2, 64), 2.0 ** 60, device="cuda", dtype=torch.bfloat16)
+    w = torch.full((64,), 2.0 ** 66, device="cuda", dtype=torch.bfloat16)
+    x[1, 9] = 2.0 ** 62
+    q, s = torch.empty(2, 64, dtype=torch.int8, device="cuda"), torch.empty(2, device="cuda")
+    ops.launch_fused_add_residual_rmsnorm_int8(w, x, None, q, s, False)
+    assert (q[0] == 127).all() and torch.isfinite(s[0]) and (q[1] == 0).all() and torch.isnan(s[1])
